@@ -263,6 +263,96 @@ int32_t turq_lm_head_topk(turq_ctx* ctx, const turq_qtensor* qt, const void* dev
                           int32_t k, int32_t id_offset, float* dev_out_vals, int32_t* dev_out_ids,
                           float* dev_logits, int32_t mode, void* stream);
 
+/* ---- Between attn_q|k|v and attn_output: head norms with rotation, the paged cache, attention
+ * (src/models/qwen3.rs:263-505: reshape, q/k RMSNorm, RoPE, KV append, attention;
+ * src/models/granite_41.rs: the same without head norms; src/models/kv_cache.rs:288-525: pages).
+ * Head dimensions are 64 or 128. Rows of q, k and v are tokens: [n_tokens, heads * head_dim] with
+ * heads side by side, `*_stride` elements from one token to the next (attn_q|k|v as views of one
+ * matrix are fine). Bases are 16-byte aligned and strides are whole multiples of 16 bytes. None of
+ * these calls allocates, synchronizes or uses memory of the context beyond its status word, so
+ * calls on different streams and replays of captured graphs do not meet in it. */
+
+/* cos and sin of position * host_freqs[i] times `scale`, computed in 64 bits: dev_table is f32
+ * [n_positions, n_freqs, 2], 16-byte aligned. n_freqs (half the rotated part of a head) is a
+ * multiple of 4, at most 64. host_freqs are read before the call returns. */
+int32_t turq_rope_table(turq_ctx* ctx, const double* host_freqs, int32_t n_freqs, int64_t n_positions, double scale,
+                        float* dev_table, void* stream);
+
+/* Per head h of every token: x = h / sqrt(mean(h^2) + eps) * weight in f32 (weights are f32
+ * [head_dim]; NULL leaves that operand's heads as they are), then the first rotary_dim (= 2 *
+ * n_freqs of the table, a multiple of 8) elements rotated by the angles of the token's position:
+ * pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0. Rounded once, to
+ * out_dtype. x_dtype and out_dtype are F32, F16 or BF16; the outputs are dense [n_tokens, heads,
+ * head_dim] and may be the inputs where type and stride agree. dev_positions are int32; one
+ * outside [0, n_positions) gives rows of zeros, and turq_ctx_poll_status then reports
+ * TURQ_E_INVALID_ARG. n_tokens = 0 is a call without work. */
+int32_t turq_qk_norm_rope(turq_ctx* ctx, const void* dev_q, int64_t q_stride, const void* dev_k, int64_t k_stride, int32_t x_dtype,
+                          int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, const float* dev_q_weight,
+                          const float* dev_k_weight, float eps, const float* dev_table, int64_t n_positions, int32_t rotary_dim,
+                          int32_t interleaved, const int32_t* dev_positions, int32_t out_dtype, void* dev_q_out, void* dev_k_out,
+                          void* stream);
+
+/* One layer's keys and values in pages of page_size tokens (a power of two, 16 to 256). dtype F16
+ * or BF16: pages are [n_pages, n_kv_heads, page_size, head_dim], keys and values apart. Q8_0: the
+ * same of int8, and an f16 scale per 32 elements in planes of their own [n_pages, n_kv_heads,
+ * page_size, head_dim / 32]. A slot is page * page_size + offset. dev_memory (256-byte aligned, at
+ * least turq_kv_cache_bytes, the caller's to keep and to free) holds the pages, or is NULL: then
+ * the handle allocates them and they read zero. Calls that read pages run in stream order behind
+ * those that write them; across streams the caller orders them. */
+typedef struct turq_kv_cache turq_kv_cache;
+size_t turq_kv_cache_bytes(int32_t dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim);
+int32_t turq_kv_cache_create(turq_ctx* ctx, int32_t dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim,
+                             void* dev_memory, size_t nbytes, turq_kv_cache** out);
+int32_t turq_kv_cache_free(turq_kv_cache* cache);
+/* Byte offsets of the four planes in the cache's memory: keys, values, scales of keys, scales of
+ * values (the last two are the total size for 16-bit types). */
+int32_t turq_kv_cache_layout(const turq_kv_cache* cache, void** dev_memory, int64_t* offsets);
+
+/* turq_qk_norm_rope with the keys, and dev_v as it is, written into the cache's slots in the same
+ * pass, rounded once or quantized: d = amax / 127 per 32 elements in f32, stored as f16, value =
+ * round-half-away(x * (1 / d)). dev_slots are int64, one per token: a negative one leaves the
+ * cache alone (padding), one past the last page too and turq_ctx_poll_status reports it. Two
+ * tokens of a call must not name one slot: what it then holds is either's, element by element. */
+int32_t turq_kv_append(turq_ctx* ctx, turq_kv_cache* cache, const void* dev_q, int64_t q_stride, const void* dev_k, int64_t k_stride,
+                       const void* dev_v, int64_t v_stride, int32_t x_dtype, int64_t n_tokens, int32_t n_q_heads,
+                       const float* dev_q_weight, const float* dev_k_weight, float eps, const float* dev_table, int64_t n_positions,
+                       int32_t rotary_dim, int32_t interleaved, const int32_t* dev_positions, const int64_t* dev_slots,
+                       int32_t out_dtype, void* dev_q_out, void* stream);
+/* Keys and values as they are into the slots (no norm, no rotation), and slots back into dense
+ * [n_tokens, n_kv_heads, head_dim] tensors of F32, F16 or BF16. Reading a negative slot, or one past
+ * the last page, gives zeros; the latter is reported. */
+int32_t turq_kv_write(turq_ctx* ctx, turq_kv_cache* cache, const void* dev_k, int64_t k_stride, const void* dev_v, int64_t v_stride,
+                      int32_t x_dtype, int64_t n_tokens, const int64_t* dev_slots, void* stream);
+int32_t turq_kv_read(turq_ctx* ctx, const turq_kv_cache* cache, const int64_t* dev_slots, int64_t n_tokens, int32_t out_dtype,
+                     void* dev_k_out, void* dev_v_out, void* stream);
+
+/* softmax(scale * q . K^T) . V of the new tokens of n_seqs sequences over their pages, n_q_heads a
+ * multiple of the cache's heads (query head h reads key head h / (n_q_heads / n_kv_heads)), at most
+ * 128 to one. Sequence i has the rows [dev_starts[i], dev_starts[i + 1]) of q (int32, ascending, n_seqs
+ * + 1 of them) and the keys in slots 0 .. dev_contexts[i] - 1 of its pages dev_page_table[i *
+ * table_stride ..] (int32), its new tokens' own keys among them as the last ones: with causal != 0
+ * the row of new token t of n sees the keys before contexts[i] - n + t + 1, otherwise all.
+ * One call takes single tokens, chunks and whole prompts together. A row that sees no key gives
+ * zeros; rows outside every sequence are left as they were.
+ * q is F16 or BF16, BF16 for a BF16 cache; out is F32, F16 or BF16, dense [n_tokens, n_q_heads,
+ * head_dim]. Products run on tensor cores in the cache's type (F16 for Q8_0) with sums, maxima
+ * and outputs held in f32. Keys and values behind a context's end may hold anything; among those
+ * of a context, values that a row does not see yet have to be finite.
+ * max_new and max_context bound what the device arrays hold; what exceeds them, an id outside the
+ * pages, or starts that descend are cut to the bounds (such a page reads as zeros) and
+ * turq_ctx_poll_status reports it. dev_workspace holds turq_kv_attention_workspace bytes (which may
+ * be 0) with the same bounds; it needs no initial value, and is the call's own until it has
+ * run: two calls that may overlap need two.
+ * For up to 16 rows per key head (new tokens x query heads to one) a row's bits do not depend on
+ * the other sequences of the call; for more, how a long context is cut goes by the whole call. */
+size_t turq_kv_attention_workspace(const turq_kv_cache* cache, int64_t n_tokens, int32_t n_seqs, int32_t n_q_heads, int64_t max_new,
+                                   int64_t max_context);
+int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void* dev_q, int64_t q_stride, int32_t q_dtype,
+                          int64_t n_tokens, int32_t n_q_heads, const int32_t* dev_starts, const int32_t* dev_contexts,
+                          const int32_t* dev_page_table, int64_t table_stride, int32_t n_seqs, int64_t max_new, int64_t max_context,
+                          float scale, int32_t causal, int32_t out_dtype, void* dev_out, void* dev_workspace, size_t workspace_bytes,
+                          void* stream);
+
 /* ---- Tensor parallelism inside one node (no counterpart in the reference, which is
  * single-device: src/models/layers/norm.rs:50 passes Shard::default() everywhere).
  *

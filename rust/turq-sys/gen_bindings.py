@@ -14,9 +14,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(HERE, "..", "..", "include", "turq.h")
 OUT = os.path.join(HERE, "src", "lib.rs")
 
-SCALARS = {"int32_t": "i32", "int64_t": "i64", "size_t": "usize", "float": "f32", "char": "c_char", "void": "c_void",
+SCALARS = {"int32_t": "i32", "int64_t": "i64", "size_t": "usize", "float": "f32", "double": "f64", "char": "c_char", "void": "c_void",
            "turq_ctx": "turq_ctx", "turq_qtensor": "turq_qtensor", "turq_tp": "turq_tp",
-           "turq_host_call": "turq_host_call"}
+           "turq_host_call": "turq_host_call", "turq_kv_cache": "turq_kv_cache"}
 
 
 def strip_comments(text: str) -> str:
@@ -101,7 +101,7 @@ def render() -> str:
            "",
            "use core::ffi::{c_char, c_void};",
            ""]
-    for name in ("turq_ctx", "turq_qtensor", "turq_tp", "turq_host_call"):
+    for name in ("turq_ctx", "turq_qtensor", "turq_tp", "turq_host_call", "turq_kv_cache"):
         out += [f"/// Opaque handle owned by the library.", "#[repr(C)]", f"pub struct {name} {{", "    _private: [u8; 0],", "}", ""]
     for name, value in consts:
         value = value.replace("(4 << 20)", "4 << 20")

@@ -30,6 +30,12 @@ pub struct turq_host_call {
     _private: [u8; 0],
 }
 
+/// Opaque handle owned by the library.
+#[repr(C)]
+pub struct turq_kv_cache {
+    _private: [u8; 0],
+}
+
 pub const TURQ_VERSION: i32 = 100;
 pub const TURQ_STATIC_SCRATCH_BYTES: usize = 4 << 20;
 pub const TURQ_TP_HANDLE_BYTES: usize = 64;
@@ -265,6 +271,141 @@ extern "C" {
         dev_out_ids: *mut i32,
         dev_logits: *mut f32,
         mode: i32,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn turq_rope_table(
+        ctx: *mut turq_ctx,
+        host_freqs: *const f64,
+        n_freqs: i32,
+        n_positions: i64,
+        scale: f64,
+        dev_table: *mut f32,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn turq_qk_norm_rope(
+        ctx: *mut turq_ctx,
+        dev_q: *const c_void,
+        q_stride: i64,
+        dev_k: *const c_void,
+        k_stride: i64,
+        x_dtype: i32,
+        n_tokens: i64,
+        n_q_heads: i32,
+        n_kv_heads: i32,
+        head_dim: i32,
+        dev_q_weight: *const f32,
+        dev_k_weight: *const f32,
+        eps: f32,
+        dev_table: *const f32,
+        n_positions: i64,
+        rotary_dim: i32,
+        interleaved: i32,
+        dev_positions: *const i32,
+        out_dtype: i32,
+        dev_q_out: *mut c_void,
+        dev_k_out: *mut c_void,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn turq_kv_cache_bytes(
+        dtype: i32,
+        n_pages: i64,
+        page_size: i32,
+        n_kv_heads: i32,
+        head_dim: i32,
+    ) -> usize;
+    pub fn turq_kv_cache_create(
+        ctx: *mut turq_ctx,
+        dtype: i32,
+        n_pages: i64,
+        page_size: i32,
+        n_kv_heads: i32,
+        head_dim: i32,
+        dev_memory: *mut c_void,
+        nbytes: usize,
+        out: *mut *mut turq_kv_cache,
+    ) -> i32;
+    pub fn turq_kv_cache_free(cache: *mut turq_kv_cache) -> i32;
+    pub fn turq_kv_cache_layout(
+        cache: *const turq_kv_cache,
+        dev_memory: *mut *mut c_void,
+        offsets: *mut i64,
+    ) -> i32;
+    pub fn turq_kv_append(
+        ctx: *mut turq_ctx,
+        cache: *mut turq_kv_cache,
+        dev_q: *const c_void,
+        q_stride: i64,
+        dev_k: *const c_void,
+        k_stride: i64,
+        dev_v: *const c_void,
+        v_stride: i64,
+        x_dtype: i32,
+        n_tokens: i64,
+        n_q_heads: i32,
+        dev_q_weight: *const f32,
+        dev_k_weight: *const f32,
+        eps: f32,
+        dev_table: *const f32,
+        n_positions: i64,
+        rotary_dim: i32,
+        interleaved: i32,
+        dev_positions: *const i32,
+        dev_slots: *const i64,
+        out_dtype: i32,
+        dev_q_out: *mut c_void,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn turq_kv_write(
+        ctx: *mut turq_ctx,
+        cache: *mut turq_kv_cache,
+        dev_k: *const c_void,
+        k_stride: i64,
+        dev_v: *const c_void,
+        v_stride: i64,
+        x_dtype: i32,
+        n_tokens: i64,
+        dev_slots: *const i64,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn turq_kv_read(
+        ctx: *mut turq_ctx,
+        cache: *const turq_kv_cache,
+        dev_slots: *const i64,
+        n_tokens: i64,
+        out_dtype: i32,
+        dev_k_out: *mut c_void,
+        dev_v_out: *mut c_void,
+        stream: *mut c_void,
+    ) -> i32;
+    pub fn turq_kv_attention_workspace(
+        cache: *const turq_kv_cache,
+        n_tokens: i64,
+        n_seqs: i32,
+        n_q_heads: i32,
+        max_new: i64,
+        max_context: i64,
+    ) -> usize;
+    pub fn turq_kv_attention(
+        ctx: *mut turq_ctx,
+        cache: *const turq_kv_cache,
+        dev_q: *const c_void,
+        q_stride: i64,
+        q_dtype: i32,
+        n_tokens: i64,
+        n_q_heads: i32,
+        dev_starts: *const i32,
+        dev_contexts: *const i32,
+        dev_page_table: *const i32,
+        table_stride: i64,
+        n_seqs: i32,
+        max_new: i64,
+        max_context: i64,
+        scale: f32,
+        causal: i32,
+        out_dtype: i32,
+        dev_out: *mut c_void,
+        dev_workspace: *mut c_void,
+        workspace_bytes: usize,
         stream: *mut c_void,
     ) -> i32;
     pub fn turq_tp_create(

@@ -53,6 +53,20 @@ SIGNATURES = {
     "turq_rmsnorm_qmatmul_multi": (c_i32, [c_vp, c_i32, c_vp, c_vp, c_i32, c_i64, c_vp, ctypes.c_float, c_vp, c_vp, c_i32, c_vp, c_vp]),
     "turq_topk": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp]),
     "turq_lm_head_topk": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp]),
+    "turq_rope_table": (c_i32, [c_vp, c_vp, c_i32, c_i64, ctypes.c_double, c_vp, c_vp]),
+    "turq_qk_norm_rope": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, ctypes.c_float,
+                                  c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_vp]),
+    "turq_kv_cache_bytes": (c_sz, [c_i32, c_i64, c_i32, c_i32, c_i32]),
+    "turq_kv_cache_create": (c_i32, [c_vp, c_i32, c_i64, c_i32, c_i32, c_i32, c_vp, c_sz, PP]),
+    "turq_kv_cache_free": (c_i32, [c_vp]),
+    "turq_kv_cache_layout": (c_i32, [c_vp, PP, ctypes.POINTER(c_i64)]),
+    "turq_kv_append": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_vp, ctypes.c_float,
+                               c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "turq_kv_write": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_vp, c_vp]),
+    "turq_kv_read": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i32, c_vp, c_vp, c_vp]),
+    "turq_kv_attention_workspace": (c_sz, [c_vp, c_i64, c_i32, c_i32, c_i64, c_i64]),
+    "turq_kv_attention": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_vp, c_vp, c_i64, c_i32, c_i64, c_i64,
+                                  ctypes.c_float, c_i32, c_i32, c_vp, c_vp, c_sz, c_vp]),
     "turq_tp_create": (c_i32, [c_vp, c_i32, c_i32, c_sz, PP]),
     "turq_tp_export": (c_i32, [c_vp, c_vp]),
     "turq_tp_connect": (c_i32, [c_vp, c_vp]),

@@ -1,0 +1,317 @@
+"""Between attn_q|k|v and attn_output: head norms with the position rotation, the paged cache of keys and
+values, and attention over it (include/turq.h, "Between attn_q|k|v and attn_output").
+
+tur does these in Qwen3Attention::forward (src/models/qwen3.rs:263-505; without head norms in
+src/models/granite_41.rs) on a PagedKvCache (src/models/kv_cache.rs:288-525). Tensors are packed: the new
+tokens of all sequences of a call stand one behind the other, [n_tokens, heads, head_dim] (or
+[n_tokens, heads * head_dim]); views with a longer stride between tokens are taken as they are.
+Every call runs on the current stream of the cache's device, allocates its outputs and workspace from
+torch and can be captured in a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from . import _lib
+from .linear import LinearX, linear
+from .quantized import (_TORCH_TO_GGML, GgmlDType, Mode, QMatMul, TurqError, _check_operand, _Context, _stream_ptr, context)
+
+_ROW_CODE = {t: int(c) for t, c in _TORCH_TO_GGML.items()}
+
+
+def _rows(x: torch.Tensor, what: str, device: int, head_dim: int) -> tuple[int, int, int]:
+    """(tokens, heads, elements from one token to the next) of a packed operand; refuses what the kernels cannot read."""
+    if not x.is_cuda or x.get_device() != device:
+        raise TurqError(1, f"{what} lives on {x.device}, expected cuda:{device}")
+    if x.dtype not in _ROW_CODE:
+        raise TurqError(3, f"{what} has dtype {x.dtype}, expected float32, float16 or bfloat16")
+    if x.dim() == 3:
+        n, heads, d = x.shape
+        dense = (d == 1 or x.stride(2) == 1) and (heads == 1 or x.stride(1) == d)
+    elif x.dim() == 2:
+        n, d = x.shape[0], head_dim
+        heads = x.shape[1] // head_dim
+        if heads * head_dim != x.shape[1]:
+            raise TurqError(2, f"{what} has {x.shape[1]} columns, not whole heads of {head_dim}")
+        dense = x.stride(1) == 1
+    else:
+        raise TurqError(2, f"{what} must be [n_tokens, heads, head_dim] or [n_tokens, heads * head_dim], got {tuple(x.shape)}")
+    if d != head_dim:
+        raise TurqError(2, f"{what} has heads of {d}, expected {head_dim}")
+    if not dense:
+        raise TurqError(1, f"{what} must hold the heads of a token side by side")
+    return n, heads, x.stride(0) if n > 1 else heads * head_dim
+
+
+def _vector(x: torch.Tensor, what: str, device: int, dtype: torch.dtype, n: Optional[int]) -> int:
+    _check_operand(x, what, device, (dtype,))
+    if n is not None and x.numel() != n:
+        raise TurqError(2, f"{what} has {x.numel()} elements, expected {n}")
+    return x.data_ptr()
+
+
+def _out(x: Optional[torch.Tensor], what: str, shape: tuple, dtype: torch.dtype, device: int) -> torch.Tensor:
+    if x is None:
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+    _check_operand(x, what, device, (dtype,))
+    if x.numel() != math.prod(shape):
+        raise TurqError(2, f"{what} has {x.numel()} elements, expected {shape}")
+    return x
+
+
+class RotaryTable:
+    """cos and sin of every position a program will use, [n_positions, rotary_dim / 2, 2] f32 on the device, computed in 64
+    bits (tur keeps the same table, src/models/qwen3.rs:64-78)."""
+
+    def __init__(self, table: torch.Tensor, rotary_dim: int, interleaved: bool, ctx: _Context):
+        self.table, self.rotary_dim, self.interleaved, self._ctx = table, rotary_dim, interleaved, ctx
+
+    @property
+    def n_positions(self) -> int:
+        return self.table.shape[0]
+
+    @classmethod
+    def new(cls, rotary_dim: int, n_positions: int, base: float = 1e6, interleaved: bool = False, scaling: Optional[dict] = None,
+            device: int | torch.device | None = None, ctx: Optional[_Context] = None) -> "RotaryTable":
+        """Frequencies base^(-2i / rotary_dim). `scaling`: {"type": "linear", "factor": f} divides every position by f;
+        {"type": "yarn", "factor": f, "original": n} does so for the slow pairs only, keeps the fast ones (pairs that turn more
+        than beta_fast = 32 times, fewer than beta_slow = 1 times over n positions, blended in between) and lengthens both by
+        0.1 ln f + 1 (the YaRN paper's rule)."""
+        if rotary_dim <= 0 or rotary_dim % 8:
+            raise TurqError(2, f"rotary_dim {rotary_dim} must be a positive multiple of 8")
+        half = rotary_dim // 2
+        freqs = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
+        scale = 1.0
+        if scaling is not None:
+            kind, factor = scaling.get("type"), float(scaling.get("factor", 1.0))
+            if factor < 1.0:
+                raise TurqError(1, f"scaling factor {factor} must be at least 1")
+            if kind == "linear":
+                freqs = [f / factor for f in freqs]
+            elif kind == "yarn":
+                n = float(scaling["original"])
+
+                def pair_of(turns: float) -> float:
+                    return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+                low = max(0, math.floor(pair_of(float(scaling.get("beta_fast", 32)))))
+                high = min(half - 1, math.ceil(pair_of(float(scaling.get("beta_slow", 1)))))
+                for i in range(half):
+                    slow = min(1.0, max(0.0, (i - low) / max(high - low, 1e-3)))
+                    freqs[i] *= 1.0 - slow + slow / factor
+                scale = 0.1 * math.log(factor) + 1.0
+            else:
+                raise TurqError(1, f"unknown scaling type {kind!r} (linear, yarn)")
+        return cls.from_frequencies(freqs, n_positions, interleaved, scale, device, ctx)
+
+    @classmethod
+    def from_frequencies(cls, freqs: Sequence[float], n_positions: int, interleaved: bool = False, scale: float = 1.0,
+                         device: int | torch.device | None = None, ctx: Optional[_Context] = None) -> "RotaryTable":
+        """Angle of pair i at a position: position * freqs[i]; cos and sin times `scale`."""
+        ctx = ctx or context(device)
+        n = len(freqs)
+        if n == 0 or n_positions <= 0:
+            raise TurqError(2, f"a table of {n} frequencies and {n_positions} positions")
+        table = torch.empty((n_positions, n, 2), dtype=torch.float32, device=torch.device("cuda", ctx.device))
+        ctx.check(_lib.load().turq_rope_table(ctx.handle, (ctypes.c_double * n)(*[float(f) for f in freqs]), n, n_positions, float(scale),
+                                              table.data_ptr(), _stream_ptr(ctx.device)))
+        return cls(table, 2 * n, bool(interleaved), ctx)
+
+
+def _rotation(q: torch.Tensor, table: RotaryTable, positions: torch.Tensor, n: int, head_dim: int, dev: int,
+              q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> tuple:
+    """The arguments from the weights to the positions, in the entries' order."""
+    if table.table.get_device() != dev:
+        raise TurqError(1, f"the rotary table lives on {table.table.device}, q on cuda:{dev}")
+    return (_vector(q_weight, "q_weight", dev, torch.float32, head_dim) if q_weight is not None else None,
+            _vector(k_weight, "k_weight", dev, torch.float32, head_dim) if k_weight is not None else None,
+            float(eps), table.table.data_ptr(), table.n_positions, table.rotary_dim, int(table.interleaved),
+            _vector(positions, "positions", dev, torch.int32, n))
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None,
+                 q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every head (where a weight is given) and rotation of q [n, heads, d] and k [n, kv_heads, d] in one pass, into
+    dense tensors of out_dtype (default: q's). positions: int32 [n]."""
+    if q.dim() != 3 or k.dim() != 3:
+        raise TurqError(2, "q and k must be [n_tokens, heads, head_dim]")
+    ctx, d = table._ctx, q.shape[-1]
+    dev = ctx.device
+    n, hq, qs = _rows(q, "q", dev, d)
+    nk, hkv, ks = _rows(k, "k", dev, d)
+    if nk != n or k.dtype != q.dtype:
+        raise TurqError(2, f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in tokens and type")
+    out_dtype = out_dtype or q.dtype
+    if out_dtype not in _ROW_CODE:
+        raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
+    qo, ko = _out(q_out, "q_out", (n, hq, d), out_dtype, dev), _out(k_out, "k_out", (n, hkv, d), out_dtype, dev)
+    st = _lib.load().turq_qk_norm_rope(ctx.handle, q.data_ptr(), qs, k.data_ptr(), ks, _ROW_CODE[q.dtype], n, hq, hkv, d,
+                                       *_rotation(q, table, positions, n, d, dev, q_weight, k_weight, eps), _ROW_CODE[out_dtype],
+                                       qo.data_ptr(), ko.data_ptr(), _stream_ptr(dev))
+    if st != 0:
+        ctx.check(st)
+    return qo, ko
+
+
+class KvCache:
+    """One layer's keys and values in pages of `page_size` tokens, 16 bits (F16, BF16) or Q8_0. A slot is page * page_size +
+    offset; which pages a sequence has is the caller's table. The memory is a torch tensor; `k_pages`, `v_pages`
+    [n_pages, n_kv_heads, page_size, head_dim] (int8 for Q8_0, with `k_scales`, `v_scales` [..., head_dim / 32]) are views of it."""
+
+    def __init__(self, handle: ctypes.c_void_p, memory: torch.Tensor, dtype: GgmlDType, shape: tuple, ctx: _Context):
+        self._h, self.memory, self.dtype, self._ctx = handle, memory, dtype, ctx
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = shape
+        off = (ctypes.c_int64 * 4)()
+        ctx.check(_lib.load().turq_kv_cache_layout(handle, None, off))
+        elem = {GgmlDType.F16: torch.float16, GgmlDType.BF16: torch.bfloat16, GgmlDType.Q8_0: torch.int8}[dtype]
+
+        def plane(o, t, last):
+            n = math.prod(shape[:3]) * last * t.itemsize
+            return memory[o:o + n].view(t).view(*shape[:3], last)
+
+        self.k_pages, self.v_pages = plane(off[0], elem, shape[3]), plane(off[1], elem, shape[3])
+        self.k_scales = self.v_scales = None
+        if dtype == GgmlDType.Q8_0:
+            self.k_scales, self.v_scales = plane(off[2], torch.float16, shape[3] // 32), plane(off[3], torch.float16, shape[3] // 32)
+
+    @classmethod
+    def new(cls, dtype: GgmlDType, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device: int | torch.device | None = None,
+            ctx: Optional[_Context] = None) -> "KvCache":
+        ctx = ctx or context(device)
+        lib = _lib.load()
+        nbytes = lib.turq_kv_cache_bytes(int(dtype), n_pages, page_size, n_kv_heads, head_dim)
+        memory = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", ctx.device))
+        h = ctypes.c_void_p()
+        ctx.check(lib.turq_kv_cache_create(ctx.handle, int(dtype), n_pages, page_size, n_kv_heads, head_dim, memory.data_ptr(), nbytes,
+                                           ctypes.byref(h)))
+        return cls(h, memory, GgmlDType(dtype), (n_pages, n_kv_heads, page_size, head_dim), ctx)
+
+    def __del__(self):
+        h, self._h = getattr(self, "_h", None), None
+        if h:
+            try:
+                _lib.load().turq_kv_cache_free(h)
+            except Exception:
+                pass
+
+    def device(self) -> torch.device:
+        return torch.device("cuda", self._ctx.device)
+
+    def _kv(self, k: torch.Tensor, v: torch.Tensor) -> tuple:
+        dev, d = self._ctx.device, self.head_dim
+        n, hk, ks = _rows(k, "k", dev, d)
+        nv, hv, vs = _rows(v, "v", dev, d)
+        if hk != self.n_kv_heads or hv != self.n_kv_heads or nv != n or v.dtype != k.dtype:
+            raise TurqError(2, f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} must agree, with {self.n_kv_heads} heads of {d}")
+        return n, ks, vs
+
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, table: RotaryTable, slots: torch.Tensor, *,
+               q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               out_dtype: torch.dtype = torch.bfloat16, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """What attn_q|k|v gave for n new tokens: norms (where a weight is given) and rotation of q and k, k and v into their
+        slots (int64 [n]; a negative one is skipped: padding), all in one pass. Returns q [n, heads, d] of out_dtype."""
+        ctx, d = self._ctx, self.head_dim
+        dev = ctx.device
+        n, ks, vs = self._kv(k, v)
+        nq, hq, qs = _rows(q, "q", dev, d)
+        if nq != n or q.dtype != k.dtype:
+            raise TurqError(2, f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in tokens and type")
+        if out_dtype not in _ROW_CODE:
+            raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
+        qo = _out(q_out, "q_out", (n, hq, d), out_dtype, dev)
+        st = _lib.load().turq_kv_append(ctx.handle, self._h, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[q.dtype], n, hq,
+                                        *_rotation(q, table, positions, n, d, dev, q_weight, k_weight, eps),
+                                        _vector(slots, "slots", dev, torch.int64, n), _ROW_CODE[out_dtype], qo.data_ptr(), _stream_ptr(dev))
+        if st != 0:
+            ctx.check(st)
+        return qo
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Keys and values as they are into their slots, rounded to the cache's type or quantized."""
+        dev = self._ctx.device
+        n, ks, vs = self._kv(k, v)
+        self._ctx.check(_lib.load().turq_kv_write(self._ctx.handle, self._h, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[k.dtype], n,
+                                                  _vector(slots, "slots", dev, torch.int64, n), _stream_ptr(dev)))
+
+    def read(self, slots: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values of the slots, [n, n_kv_heads, d] each; a negative slot reads as zeros."""
+        dev, n = self._ctx.device, slots.numel()
+        if out_dtype not in _ROW_CODE:
+            raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
+        k, v = (_out(None, "", (n, self.n_kv_heads, self.head_dim), out_dtype, dev) for _ in range(2))
+        self._ctx.check(_lib.load().turq_kv_read(self._ctx.handle, self._h, _vector(slots, "slots", dev, torch.int64, None), n,
+                                                 _ROW_CODE[out_dtype], k.data_ptr(), v.data_ptr(), _stream_ptr(dev)))
+        return k, v
+
+    def attend(self, q: torch.Tensor, starts: torch.Tensor, contexts: torch.Tensor, page_table: torch.Tensor, *, max_new: Optional[int] = None,
+               max_context: Optional[int] = None, scale: Optional[float] = None, causal: bool = True,
+               out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """softmax(scale q K^T) V of the new tokens of n_seqs sequences over their pages: q [n, heads, d] packed, rows
+        starts[i] .. starts[i + 1] (int32 [n_seqs + 1]) of sequence i, whose context of contexts[i] tokens (int32 [n_seqs], the new
+        ones last) lies in the pages page_table[i] (int32 [n_seqs, pages]). scale: 1 / sqrt(d) by default. Single tokens,
+        chunks and whole prompts go together; max_new and max_context are the longest of each that the call may meet (the
+        values on the device are not read here). `out` keeps its rows that belong to no sequence."""
+        ctx, d = self._ctx, self.head_dim
+        dev = ctx.device
+        n, hq, qs = _rows(q, "q", dev, d)
+        _check_operand(page_table, "page_table", dev, (torch.int32,))
+        if page_table.dim() != 2:
+            raise TurqError(2, f"page_table must be [n_seqs, pages], got {tuple(page_table.shape)}")
+        n_seqs, pages = page_table.shape
+        p_starts = _vector(starts, "starts", dev, torch.int32, n_seqs + 1)
+        p_contexts = _vector(contexts, "contexts", dev, torch.int32, n_seqs)
+        max_new = n if max_new is None else int(max_new)
+        max_context = pages * self.page_size if max_context is None else int(max_context)
+        out_dtype = (out.dtype if out is not None else q.dtype) if out_dtype is None else out_dtype
+        if out_dtype not in _ROW_CODE:
+            raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
+        y = _out(out, "out", (n, hq, d), out_dtype, dev)
+        lib = _lib.load()
+        nbytes = lib.turq_kv_attention_workspace(self._h, n, n_seqs, hq, max_new, max_context)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=y.device).data_ptr() if nbytes else None
+        st = lib.turq_kv_attention(ctx.handle, self._h, q.data_ptr(), qs, _ROW_CODE[q.dtype], n, hq, p_starts, p_contexts, page_table.data_ptr(),
+                                   pages, n_seqs, max_new, max_context, 1.0 / math.sqrt(d) if scale is None else float(scale), int(causal),
+                                   _ROW_CODE[out_dtype], y.data_ptr(), ws, nbytes, _stream_ptr(dev))
+        if st != 0:
+            ctx.check(st)
+        return y if y.dim() == 3 else y.view(n, hq, d)
+
+
+class Attention:
+    """tur's attention block on a quantized layer (Qwen3Attention, src/models/qwen3.rs:205-222, 263-505; Granite's without
+    head norms): attn_q|k|v in one call, norms, rotation and cache write in one pass, attention, attn_output."""
+
+    def __init__(self, q: LinearX, k: LinearX, v: LinearX, o: LinearX, head_dim: int, q_norm: Optional[torch.Tensor] = None,
+                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, scale: Optional[float] = None):
+        self.q, self.k, self.v, self.o = q, k, v, o
+        self.head_dim, self.q_norm, self.k_norm, self.eps, self.scale = head_dim, q_norm, k_norm, eps, scale
+
+    @classmethod
+    def new(cls, vb, hidden: int, n_heads: int, n_kv_heads: int, head_dim: int, eps: float = 1e-6, scale: Optional[float] = None) -> "Attention":
+        """From the tensors of one block (`vb.pp("blk").pp(i)`): attn_q, attn_k, attn_v, attn_output, and attn_q_norm /
+        attn_k_norm where the file has them."""
+        def norm(name):
+            return vb.pp(name).get(head_dim, "weight").dequantize().reshape(head_dim) if vb.pp(name).contains_key("weight") else None
+
+        return cls(linear(hidden, n_heads * head_dim, vb.pp("attn_q")), linear(hidden, n_kv_heads * head_dim, vb.pp("attn_k")),
+                   linear(hidden, n_kv_heads * head_dim, vb.pp("attn_v")), linear(n_heads * head_dim, hidden, vb.pp("attn_output")),
+                   head_dim, norm("attn_q_norm"), norm("attn_k_norm"), eps, scale)
+
+    def forward(self, x: torch.Tensor, cache: KvCache, table: RotaryTable, positions: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor,
+                contexts: torch.Tensor, page_table: torch.Tensor, *, max_new: Optional[int] = None, max_context: Optional[int] = None,
+                mode: Mode = Mode.AUTO) -> torch.Tensor:
+        """x [n_tokens, hidden] (f32 or bf16), the packed new tokens of all sequences -> [n_tokens, hidden] f32. The other
+        arguments are those of KvCache.append and KvCache.attend."""
+        linears = (self.q, self.k, self.v)
+        biases = [l.bias for l in linears] if any(l.bias is not None for l in linears) else None
+        q, k, v = QMatMul.forward_multi([l.qmatmul for l in linears], x, biases=biases, mode=mode)
+        q = cache.append(q, k, v, positions, table, slots, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.eps)
+        y = cache.attend(q, starts, contexts, page_table, max_new=max_new, max_context=max_context, scale=self.scale)
+        return self.o.forward(y.view(y.shape[0], -1), mode=mode)
+
+    __call__ = forward

@@ -49,3 +49,14 @@ struct turq_host_call {
   uint8_t* scratch = nullptr;
   cudaGraphExec_t exec = nullptr;
 };
+
+// One layer's keys and values in pages (turq_kv_cache_*): four planes in one piece of memory.
+struct turq_kv_cache {
+  int device = 0;
+  int dtype = 0;
+  int64_t n_pages = 0;
+  int page_size = 0, n_kv_heads = 0, head_dim = 0;
+  uint8_t* mem = nullptr;
+  bool owns = false;
+  size_t off_k = 0, off_v = 0, off_ks = 0, off_vs = 0, bytes = 0;
+};

@@ -1,0 +1,512 @@
+// Between attn_q|k|v and attention: norms of the heads with the position rotation, and the paged cache of
+// keys and values that takes them (src/models/qwen3.rs:263-305; src/models/kv_cache.rs:288-525).
+//   * rope_table_kernel: cos / sin of position x frequency, in 64 bits (far positions lose their angle in
+//     32: a position of 1e5 is known to 4e-3 of a turn's radian there);
+//   * head_rows_kernel: one pass over the rows of q, k and v. A row is one head of one token; x / sqrt(mean(x^2)
+//     + eps) * w and the rotation are done in registers, and the row goes to a dense tensor or to its page,
+//     rounded once or quantized to Q8_0;
+//   * kv_read_kernel: slots back into dense rows.
+#include <new>
+
+#include "../../include/turq.h"
+#include "actquant.cuh"
+#include "device_utils.cuh"
+#include "handles.h"
+#include "kvcache.cuh"
+#include "turq_internal.h"
+
+namespace turq {
+
+struct Frequencies { double f[64]; };
+
+__global__ void __launch_bounds__(256) rope_table_kernel(const Frequencies fr, int n_freqs, int64_t total, double scale, float2* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    double s, c;
+    sincos((double)(i / n_freqs) * fr.f[i % n_freqs], &s, &c);
+    out[i] = make_float2((float)(c * scale), (float)(s * scale));
+  }
+}
+
+// Four neighbouring elements of a row, whatever their type.
+__device__ __forceinline__ void load4(const void* p, int dtype, int64_t i, float (&v)[4]) {
+  if (dtype == TURQ_F32) {
+    const float4 t = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    return;
+  }
+  const uint2 t = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+  float2 a, b;
+  if (dtype == TURQ_BF16) {
+    a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&t.x));
+    b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&t.y));
+  } else {
+    a = __half22float2(*reinterpret_cast<const __half2*>(&t.x));
+    b = __half22float2(*reinterpret_cast<const __half2*>(&t.y));
+  }
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const float* v) {
+  if (dtype == TURQ_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    return;
+  }
+  uint2 t;
+  if (dtype == TURQ_BF16) {
+    *reinterpret_cast<__nv_bfloat162*>(&t.x) = __floats2bfloat162_rn(v[0], v[1]);
+    *reinterpret_cast<__nv_bfloat162*>(&t.y) = __floats2bfloat162_rn(v[2], v[3]);
+  } else {
+    *reinterpret_cast<__half2*>(&t.x) = __floats2half2_rn(v[0], v[1]);
+    *reinterpret_cast<__half2*>(&t.y) = __floats2half2_rn(v[2], v[3]);
+  }
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = t;
+}
+
+struct HeadRowsArgs {
+  const void *q, *k, *v;            // v: only with a cache
+  int64_t q_stride, k_stride, v_stride;
+  int x_dtype, out_dtype;
+  int64_t n_tokens;
+  int hq, hkv;                      // hq = 0: keys and values alone
+  const float *wq, *wk;
+  float eps;
+  const float2* table;              // null: no rotation
+  int64_t n_positions;
+  int half_rot, interleaved;
+  const int32_t* positions;
+  void *q_out, *k_out;              // k_out: without a cache
+  KvPages cache;                    // cache.k null: none
+  const int64_t* slots;
+  int* status;
+};
+
+// D / 8 lanes hold a row, eight elements each: a lane owns four pairs, so the rotation stays in its
+// registers. Pair p of the rotated part is (p, p + half_rot), or (2p, 2p + 1) interleaved; behind it
+// lane j simply has elements 8j .. 8j + 7. half_rot is a multiple of 4: no lane straddles the border.
+template <int D>
+__global__ void __launch_bounds__(256) head_rows_kernel(const HeadRowsArgs a) {
+  constexpr int L = D / 8;
+  const int j = threadIdx.x % L;
+  const int rows_per_token = a.hq + a.hkv * (a.cache.k ? 2 : 1);
+  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  // Lanes of rows that do not exist stay: the rows of a warp reduce together.
+  const bool live = row < a.n_tokens * rows_per_token;
+  const int64_t token = live ? row / rows_per_token : 0;
+  const int r = live ? (int)(row % rows_per_token) : 0;
+  const bool is_q = r < a.hq, is_v = r >= a.hq + a.hkv;
+  const int h = is_q ? r : is_v ? r - a.hq - a.hkv : r - a.hq;
+  const bool turn = a.table != nullptr && !is_v && 4 * j < a.half_rot;
+  const bool split = turn && !a.interleaved;       // this lane's pairs lie half_rot apart
+  const int e0 = split ? 4 * j : 8 * j, e1 = split ? a.half_rot + 4 * j : 8 * j + 4;
+
+  float x[8];
+  const void* src = is_q ? a.q : is_v ? a.v : a.k;
+  const int64_t base = token * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) + (int64_t)h * D;
+  load4(src, a.x_dtype, base + e0, reinterpret_cast<float(&)[4]>(x[0]));
+  load4(src, a.x_dtype, base + e1, reinterpret_cast<float(&)[4]>(x[4]));
+  int64_t pos = 0;
+  bool known = true;
+  if (a.table) {
+    pos = a.positions[token];
+    known = pos >= 0 && pos < a.n_positions;
+    if (!known && live) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
+  }
+  const float* w = is_q ? a.wq : is_v ? nullptr : a.wk;
+  if (a.wq || a.wk) {  // the whole grid the same way: the shuffles need every lane
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) ss += x[e] * x[e];
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+    if (w) {
+      const float rms = sqrtf(ss / D + a.eps);
+      float wv[8];
+      load4(w, TURQ_F32, e0, reinterpret_cast<float(&)[4]>(wv[0]));
+      load4(w, TURQ_F32, e1, reinterpret_cast<float(&)[4]>(wv[4]));
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = x[e] / rms * wv[e];
+    }
+  }
+  if (turn && known) {
+    const float4* t = reinterpret_cast<const float4*>(a.table + pos * a.half_rot + 4 * j);
+    const float4 t0 = t[0], t1 = t[1];
+    const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float& p = split ? x[i] : x[2 * i];
+      float& q = split ? x[4 + i] : x[2 * i + 1];
+      const float px = p, qx = q;
+      p = px * c[i] - qx * s[i];
+      q = qx * c[i] + px * s[i];
+    }
+  }
+  if (!known) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = 0.f;
+  }
+
+  if (is_q || !a.cache.k) {
+    if (live) {
+      void* out = is_q ? a.q_out : a.k_out;
+      const int64_t o = (token * (is_q ? a.hq : a.hkv) + h) * D;
+      store4(out, a.out_dtype, o + e0, x);
+      store4(out, a.out_dtype, o + e1, x + 4);
+    }
+    if (!a.cache.k) return;
+  }
+  const int64_t slot = live && !is_q ? a.slots[token] : -1;
+  const bool fits = slot < a.cache.n_pages * a.cache.page_size;
+  if (!fits) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
+  const bool write = live && !is_q && slot >= 0 && fits && known;
+  const int64_t at = write ? a.cache.row(slot, h) : 0;  // row of the planes
+  if (a.cache.dtype != TURQ_Q8_0) {
+    if (write) {
+      void* out = is_v ? a.cache.v : a.cache.k;
+      store4(out, a.cache.dtype, at * D + e0, x);
+      store4(out, a.cache.dtype, at * D + e1, x + 4);
+    }
+    return;
+  }
+  // Q8_0: lane j gets elements 8j .. 8j + 7, so that four lanes hold a block of 32. A group of four
+  // elements 4g .. 4g + 3 of a row whose pairs lie apart is the first half of lane g's registers, the second
+  // half of lane g - half_rot / 4's, or one of the two of lane g / 2.
+  if (a.table && !a.interleaved) {
+    float y[8];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const int g = 2 * j + b, q4 = a.half_rot / 4;
+      const bool apart = a.table && !is_v;
+      const int from = apart && g < q4 ? g : apart && g < 2 * q4 ? g - q4 : g / 2;
+      const bool second = apart && g < q4 ? false : apart && g < 2 * q4 ? true : (g & 1) != 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float lo = __shfl_sync(0xFFFFFFFFu, x[i], from, L), hi = __shfl_sync(0xFFFFFFFFu, x[4 + i], from, L);
+        y[4 * b + i] = second ? hi : lo;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = y[e];
+  }
+  uint32_t w0, w1;
+  __half d;
+  quant_block_q8_0(x, w0, w1, d);
+  if (!write) return;
+  *reinterpret_cast<uint2*>((is_v ? a.cache.v : a.cache.k) + at * D + 8 * j) = make_uint2(w0, w1);
+  if ((j & 3) == 0) (is_v ? a.cache.vs : a.cache.ks)[at * (D / 32) + j / 4] = d;
+}
+
+// A group of D / 8 lanes per row of keys or values.
+template <int D>
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvPages c, const int64_t* __restrict__ slots, int64_t n_tokens, int out_dtype,
+                                                      void* __restrict__ k_out, void* __restrict__ v_out, int* status) {
+  constexpr int L = D / 8;
+  const int j = threadIdx.x % L;
+  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (row >= 2 * n_tokens * c.n_heads) return;
+  const int64_t token = row / (2 * c.n_heads);
+  const int h = (int)(row % c.n_heads);
+  const bool is_v = row % (2 * c.n_heads) >= c.n_heads;
+  const int64_t slot = slots[token];
+  const bool fits = slot < c.n_pages * c.page_size;
+  if (!fits) *reinterpret_cast<volatile int*>(status) = TURQ_E_INVALID_ARG;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (slot >= 0 && fits) {
+    const int64_t at = c.row(slot, h);
+    const uint8_t* src = is_v ? c.v : c.k;
+    if (c.dtype == TURQ_Q8_0) {
+      const float d = __half2float((is_v ? c.vs : c.ks)[at * (D / 32) + j / 4]);
+      const uint2 t = *reinterpret_cast<const uint2*>(src + at * D + 8 * j);
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = d * (float)(int8_t)((e < 4 ? t.x : t.y) >> (8 * (e & 3)));
+    } else {
+      load4(src, c.dtype, at * D + 8 * j, reinterpret_cast<float(&)[4]>(x[0]));
+      load4(src, c.dtype, at * D + 8 * j + 4, reinterpret_cast<float(&)[4]>(x[4]));
+    }
+  }
+  void* out = is_v ? v_out : k_out;
+  const int64_t o = (token * c.n_heads + h) * D + 8 * j;
+  store4(out, out_dtype, o, x);
+  store4(out, out_dtype, o + 4, x + 4);
+}
+
+static cudaError_t launch_head_rows(int head_dim, const HeadRowsArgs& a, cudaStream_t s) {
+  const int64_t rows = a.n_tokens * (a.hq + a.hkv * (a.cache.k ? 2 : 1));
+  const int per_block = 256 / (head_dim / 8);
+  const unsigned grid = (unsigned)((rows + per_block - 1) / per_block);
+  if (head_dim == 64) head_rows_kernel<64><<<grid, 256, 0, s>>>(a);
+  else head_rows_kernel<128><<<grid, 256, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace turq
+
+namespace {
+
+using turq::api_cuda_fail;
+using turq::api_fail;
+
+int32_t elem_bytes(int32_t dtype) { return dtype == TURQ_F32 ? 4 : dtype == TURQ_F16 || dtype == TURQ_BF16 ? 2 : 0; }
+
+// An operand of rows: base and stride in whole 16 bytes, rows that do not overlap.
+int32_t check_rows(turq_ctx* ctx, const void* p, int64_t stride, int64_t width, int32_t dtype) {
+  if (!p) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if (stride < width) return api_fail(ctx, TURQ_E_SHAPE, "the stride of q, k or v is less than the width of its heads");
+  if ((uintptr_t)p % 16 != 0 || stride * elem_bytes(dtype) % 16 != 0)
+    return api_fail(ctx, TURQ_E_ALIGN, "q, k and v need 16-byte aligned bases and strides of whole 16 bytes");
+  return TURQ_OK;
+}
+
+int32_t check_tokens(turq_ctx* ctx, int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return api_fail(ctx, TURQ_E_SHAPE, "head_dim must be 64 or 128");
+  if (n_q_heads < 0 || n_kv_heads < 1 || n_q_heads > 65536 || n_kv_heads > 65536) return api_fail(ctx, TURQ_E_SHAPE, "head counts must be in 1..65536");
+  // one launch of 8 or 16 rows a block
+  if (n_tokens < 0 || n_tokens > INT32_MAX / 2 || n_tokens * ((int64_t)n_q_heads + 2 * (int64_t)n_kv_heads) > (int64_t)INT32_MAX * 8)
+    return api_fail(ctx, TURQ_E_SHAPE, "n_tokens out of range");
+  return TURQ_OK;
+}
+
+// Norm weights, table and positions of a rotating call.
+int32_t check_rotation(turq_ctx* ctx, const float* wq, const float* wk, const float* table, int64_t n_positions, int32_t rotary_dim,
+                       int32_t head_dim, const int32_t* positions) {
+  if (!table || !positions) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if (rotary_dim <= 0 || rotary_dim > head_dim || rotary_dim % 8 != 0) return api_fail(ctx, TURQ_E_SHAPE, "rotary_dim must be a multiple of 8 up to head_dim");
+  if (n_positions <= 0) return api_fail(ctx, TURQ_E_SHAPE, "the table has no positions");
+  if ((uintptr_t)table % 16 != 0 || (uintptr_t)wq % 16 != 0 || (uintptr_t)wk % 16 != 0 || (uintptr_t)positions % 4 != 0)
+    return api_fail(ctx, TURQ_E_ALIGN, "table and norm weights must be 16-byte, positions 4-byte aligned");
+  return TURQ_OK;
+}
+
+int32_t check_cache(turq_ctx* ctx, const turq_kv_cache* cache, const void* slots) {
+  if (cache->device != ctx->device) return api_fail(ctx, TURQ_E_INVALID_ARG, "cache and context must live on the same device");
+  if (!slots) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if ((uintptr_t)slots % 8 != 0) return api_fail(ctx, TURQ_E_ALIGN, "slots must be 8-byte aligned");
+  return TURQ_OK;
+}
+
+#define TQ_TRY(expr)                      \
+  do {                                    \
+    const int32_t st__ = (expr);          \
+    if (st__ != TURQ_OK) return st__;     \
+  } while (0)
+
+int32_t run_head_rows(turq_ctx* ctx, int head_dim, const turq::HeadRowsArgs& a, void* stream, const char* what) {
+  turq::DeviceScope on(ctx->device);
+  cudaError_t e = on.status;
+  if (e == cudaSuccess) e = turq::launch_head_rows(head_dim, a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return api_cuda_fail(ctx, e, what);
+  ctx->launches++;
+  return TURQ_OK;
+}
+
+struct CacheShape { size_t off_v, off_ks, off_vs, bytes; bool ok; };
+CacheShape cache_shape(int32_t dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim) {
+  CacheShape c{0, 0, 0, 0, false};
+  if (dtype != TURQ_F16 && dtype != TURQ_BF16 && dtype != TURQ_Q8_0) return c;
+  if (head_dim != 64 && head_dim != 128) return c;
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0) return c;
+  if (n_pages <= 0 || n_kv_heads <= 0 || n_kv_heads > 65536 || n_pages > INT32_MAX / n_kv_heads) return c;  // page x head is a 31-bit index
+  auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+  const size_t rows = (size_t)n_pages * n_kv_heads * page_size;
+  const size_t plane = up(rows * head_dim * (dtype == TURQ_Q8_0 ? 1 : 2)), scales = dtype == TURQ_Q8_0 ? up(rows * (head_dim / 32) * 2) : 0;
+  c.off_v = plane;
+  c.off_ks = 2 * plane;
+  c.off_vs = 2 * plane + scales;
+  c.bytes = 2 * plane + 2 * scales;
+  c.ok = true;
+  return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t turq_rope_table(turq_ctx* ctx, const double* host_freqs, int32_t n_freqs, int64_t n_positions, double scale, float* dev_table, void* stream) {
+  if (!ctx || !host_freqs || !dev_table) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if (n_freqs <= 0 || n_freqs > 64 || n_freqs % 4 != 0) return api_fail(ctx, TURQ_E_SHAPE, "n_freqs must be a multiple of 4, at most 64");
+  if (n_positions <= 0 || n_positions > INT32_MAX) return api_fail(ctx, TURQ_E_SHAPE, "n_positions out of range");
+  if ((uintptr_t)dev_table % 16 != 0) return api_fail(ctx, TURQ_E_ALIGN, "dev_table must be 16-byte aligned");
+  turq::Frequencies fr{};
+  for (int i = 0; i < n_freqs; i++) fr.f[i] = host_freqs[i];
+  turq::DeviceScope on(ctx->device);
+  if (on.status != cudaSuccess) return api_cuda_fail(ctx, on.status, "rope table launch");
+  const int64_t total = n_positions * n_freqs;
+  int64_t blocks = (total + 255) / 256;
+  if (blocks > 32 * (int64_t)ctx->sm_count) blocks = 32 * (int64_t)ctx->sm_count;
+  turq::rope_table_kernel<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(fr, n_freqs, total, scale, reinterpret_cast<float2*>(dev_table));
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return api_cuda_fail(ctx, e, "rope table launch");
+  ctx->launches++;
+  return TURQ_OK;
+}
+
+int32_t turq_qk_norm_rope(turq_ctx* ctx, const void* dev_q, int64_t q_stride, const void* dev_k, int64_t k_stride, int32_t x_dtype,
+                          int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, const float* dev_q_weight,
+                          const float* dev_k_weight, float eps, const float* dev_table, int64_t n_positions, int32_t rotary_dim,
+                          int32_t interleaved, const int32_t* dev_positions, int32_t out_dtype, void* dev_q_out, void* dev_k_out,
+                          void* stream) {
+  if (!ctx) return TURQ_E_INVALID_ARG;
+  if (!elem_bytes(x_dtype) || !elem_bytes(out_dtype)) return api_fail(ctx, TURQ_E_DTYPE, "rows must be F32, F16 or BF16");
+  TQ_TRY(check_tokens(ctx, n_tokens, n_q_heads, n_kv_heads, head_dim));
+  if (n_q_heads < 1) return api_fail(ctx, TURQ_E_SHAPE, "head counts must be in 1..65536");
+  if (n_tokens == 0) return TURQ_OK;
+  TQ_TRY(check_rows(ctx, dev_q, q_stride, (int64_t)n_q_heads * head_dim, x_dtype));
+  TQ_TRY(check_rows(ctx, dev_k, k_stride, (int64_t)n_kv_heads * head_dim, x_dtype));
+  TQ_TRY(check_rotation(ctx, dev_q_weight, dev_k_weight, dev_table, n_positions, rotary_dim, head_dim, dev_positions));
+  if (!dev_q_out || !dev_k_out) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if ((uintptr_t)dev_q_out % 16 != 0 || (uintptr_t)dev_k_out % 16 != 0) return api_fail(ctx, TURQ_E_ALIGN, "outputs must be 16-byte aligned");
+  turq::HeadRowsArgs a{};
+  a.q = dev_q; a.k = dev_k;
+  a.q_stride = q_stride; a.k_stride = k_stride;
+  a.x_dtype = x_dtype; a.out_dtype = out_dtype;
+  a.n_tokens = n_tokens; a.hq = n_q_heads; a.hkv = n_kv_heads;
+  a.wq = dev_q_weight; a.wk = dev_k_weight; a.eps = eps;
+  a.table = reinterpret_cast<const float2*>(dev_table); a.n_positions = n_positions;
+  a.half_rot = rotary_dim / 2; a.interleaved = interleaved != 0; a.positions = dev_positions;
+  a.q_out = dev_q_out; a.k_out = dev_k_out;
+  a.status = ctx->dev_status;
+  return run_head_rows(ctx, head_dim, a, stream, "qk_norm_rope launch");
+}
+
+size_t turq_kv_cache_bytes(int32_t dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim) {
+  const CacheShape c = cache_shape(dtype, n_pages, page_size, n_kv_heads, head_dim);
+  return c.ok ? c.bytes : 0;
+}
+
+int32_t turq_kv_cache_create(turq_ctx* ctx, int32_t dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim,
+                             void* dev_memory, size_t nbytes, turq_kv_cache** out) {
+  if (!ctx || !out) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  *out = nullptr;
+  if (dtype != TURQ_F16 && dtype != TURQ_BF16 && dtype != TURQ_Q8_0) return api_fail(ctx, TURQ_E_DTYPE, "a cache holds F16, BF16 or Q8_0");
+  const CacheShape c = cache_shape(dtype, n_pages, page_size, n_kv_heads, head_dim);
+  if (!c.ok)
+    return api_fail(ctx, TURQ_E_SHAPE, "a cache needs head_dim 64 or 128, pages of 16 to 256 tokens (a power of two), and n_pages * n_kv_heads in 31 bits");
+  if (dev_memory && nbytes < c.bytes) return api_fail(ctx, TURQ_E_SHAPE, "dev_memory holds less than turq_kv_cache_bytes");
+  if ((uintptr_t)dev_memory % 256 != 0) return api_fail(ctx, TURQ_E_ALIGN, "dev_memory must be 256-byte aligned");
+  turq::DeviceScope on(ctx->device);
+  if (on.status != cudaSuccess) return api_cuda_fail(ctx, on.status, "cudaSetDevice");
+  turq_kv_cache* kc = new (std::nothrow) turq_kv_cache();
+  if (!kc) return api_fail(ctx, TURQ_E_INVALID_ARG, "out of host memory");
+  kc->device = ctx->device;
+  kc->dtype = dtype;
+  kc->n_pages = n_pages;
+  kc->page_size = page_size;
+  kc->n_kv_heads = n_kv_heads;
+  kc->head_dim = head_dim;
+  kc->off_v = c.off_v;
+  kc->off_ks = c.off_ks;
+  kc->off_vs = c.off_vs;
+  kc->bytes = c.bytes;
+  kc->mem = static_cast<uint8_t*>(dev_memory);
+  if (!dev_memory) {
+    cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&kc->mem), c.bytes);
+    kc->owns = e == cudaSuccess;
+    if (e == cudaSuccess) e = cudaMemset(kc->mem, 0, c.bytes);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      turq_kv_cache_free(kc);
+      return api_cuda_fail(ctx, e, "allocating the cache's pages");
+    }
+  }
+  *out = kc;
+  return TURQ_OK;
+}
+
+int32_t turq_kv_cache_free(turq_kv_cache* cache) {
+  if (!cache) return TURQ_E_INVALID_ARG;
+  if (cache->owns) {
+    turq::DeviceScope on(cache->device);
+    cudaFree(cache->mem);
+  }
+  delete cache;
+  return TURQ_OK;
+}
+
+int32_t turq_kv_cache_layout(const turq_kv_cache* cache, void** dev_memory, int64_t* offsets) {
+  if (!cache) return TURQ_E_INVALID_ARG;
+  if (dev_memory) *dev_memory = cache->mem;
+  if (offsets) {
+    offsets[0] = 0;
+    offsets[1] = (int64_t)cache->off_v;
+    offsets[2] = (int64_t)cache->off_ks;
+    offsets[3] = (int64_t)cache->off_vs;
+  }
+  return TURQ_OK;
+}
+
+int32_t turq_kv_append(turq_ctx* ctx, turq_kv_cache* cache, const void* dev_q, int64_t q_stride, const void* dev_k, int64_t k_stride,
+                       const void* dev_v, int64_t v_stride, int32_t x_dtype, int64_t n_tokens, int32_t n_q_heads,
+                       const float* dev_q_weight, const float* dev_k_weight, float eps, const float* dev_table, int64_t n_positions,
+                       int32_t rotary_dim, int32_t interleaved, const int32_t* dev_positions, const int64_t* dev_slots,
+                       int32_t out_dtype, void* dev_q_out, void* stream) {
+  if (!ctx || !cache) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if (!elem_bytes(x_dtype) || !elem_bytes(out_dtype)) return api_fail(ctx, TURQ_E_DTYPE, "rows must be F32, F16 or BF16");
+  const int d = cache->head_dim, hkv = cache->n_kv_heads;
+  TQ_TRY(check_tokens(ctx, n_tokens, n_q_heads, hkv, d));
+  if (n_q_heads < 1) return api_fail(ctx, TURQ_E_SHAPE, "head counts must be in 1..65536");
+  if (n_tokens == 0) return TURQ_OK;
+  TQ_TRY(check_rows(ctx, dev_q, q_stride, (int64_t)n_q_heads * d, x_dtype));
+  TQ_TRY(check_rows(ctx, dev_k, k_stride, (int64_t)hkv * d, x_dtype));
+  TQ_TRY(check_rows(ctx, dev_v, v_stride, (int64_t)hkv * d, x_dtype));
+  TQ_TRY(check_rotation(ctx, dev_q_weight, dev_k_weight, dev_table, n_positions, rotary_dim, d, dev_positions));
+  TQ_TRY(check_cache(ctx, cache, dev_slots));
+  if (!dev_q_out) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if ((uintptr_t)dev_q_out % 16 != 0) return api_fail(ctx, TURQ_E_ALIGN, "outputs must be 16-byte aligned");
+  turq::HeadRowsArgs a{};
+  a.q = dev_q; a.k = dev_k; a.v = dev_v;
+  a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+  a.x_dtype = x_dtype; a.out_dtype = out_dtype;
+  a.n_tokens = n_tokens; a.hq = n_q_heads; a.hkv = hkv;
+  a.wq = dev_q_weight; a.wk = dev_k_weight; a.eps = eps;
+  a.table = reinterpret_cast<const float2*>(dev_table); a.n_positions = n_positions;
+  a.half_rot = rotary_dim / 2; a.interleaved = interleaved != 0; a.positions = dev_positions;
+  a.q_out = dev_q_out;
+  a.cache = turq::pages_of(cache); a.slots = dev_slots;
+  a.status = ctx->dev_status;
+  return run_head_rows(ctx, d, a, stream, "kv_append launch");
+}
+
+int32_t turq_kv_write(turq_ctx* ctx, turq_kv_cache* cache, const void* dev_k, int64_t k_stride, const void* dev_v, int64_t v_stride,
+                      int32_t x_dtype, int64_t n_tokens, const int64_t* dev_slots, void* stream) {
+  if (!ctx || !cache) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if (!elem_bytes(x_dtype)) return api_fail(ctx, TURQ_E_DTYPE, "rows must be F32, F16 or BF16");
+  const int d = cache->head_dim, hkv = cache->n_kv_heads;
+  TQ_TRY(check_tokens(ctx, n_tokens, 0, hkv, d));
+  if (n_tokens == 0) return TURQ_OK;
+  TQ_TRY(check_rows(ctx, dev_k, k_stride, (int64_t)hkv * d, x_dtype));
+  TQ_TRY(check_rows(ctx, dev_v, v_stride, (int64_t)hkv * d, x_dtype));
+  TQ_TRY(check_cache(ctx, cache, dev_slots));
+  turq::HeadRowsArgs a{};
+  a.k = dev_k; a.v = dev_v;
+  a.k_stride = k_stride; a.v_stride = v_stride;
+  a.x_dtype = x_dtype;
+  a.n_tokens = n_tokens; a.hkv = hkv;
+  a.cache = turq::pages_of(cache); a.slots = dev_slots;
+  a.status = ctx->dev_status;
+  return run_head_rows(ctx, d, a, stream, "kv_write launch");
+}
+
+int32_t turq_kv_read(turq_ctx* ctx, const turq_kv_cache* cache, const int64_t* dev_slots, int64_t n_tokens, int32_t out_dtype,
+                     void* dev_k_out, void* dev_v_out, void* stream) {
+  if (!ctx || !cache) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if (!elem_bytes(out_dtype)) return api_fail(ctx, TURQ_E_DTYPE, "rows must be F32, F16 or BF16");
+  const int d = cache->head_dim, hkv = cache->n_kv_heads;
+  TQ_TRY(check_tokens(ctx, n_tokens, 0, hkv, d));
+  if (n_tokens == 0) return TURQ_OK;
+  TQ_TRY(check_cache(ctx, cache, dev_slots));
+  if (!dev_k_out || !dev_v_out) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
+  if ((uintptr_t)dev_k_out % 16 != 0 || (uintptr_t)dev_v_out % 16 != 0) return api_fail(ctx, TURQ_E_ALIGN, "outputs must be 16-byte aligned");
+  turq::DeviceScope on(ctx->device);
+  if (on.status != cudaSuccess) return api_cuda_fail(ctx, on.status, "kv_read launch");
+  const turq::KvPages pages = turq::pages_of(cache);
+  const int per_block = 256 / (d / 8);
+  const unsigned grid = (unsigned)((2 * n_tokens * hkv + per_block - 1) / per_block);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (d == 64) turq::kv_read_kernel<64><<<grid, 256, 0, s>>>(pages, dev_slots, n_tokens, out_dtype, dev_k_out, dev_v_out, ctx->dev_status);
+  else turq::kv_read_kernel<128><<<grid, 256, 0, s>>>(pages, dev_slots, n_tokens, out_dtype, dev_k_out, dev_v_out, ctx->dev_status);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return api_cuda_fail(ctx, e, "kv_read launch");
+  ctx->launches++;
+  return TURQ_OK;
+}
+
+}  // extern "C"
