@@ -3,46 +3,11 @@
 // running maximum m and sum.
 #include <cfloat>
 
-#include "../../include/turq.h"
-#include "device_utils.cuh"
-#include "handles.h"
-#include "kvcache.cuh"
+#include "attend.cuh"
+#include "attend_launch.h"
 #include "turq_internal.h"
 
 namespace turq {
-
-struct AttendArgs {
-  KvPages cache;
-  const uint16_t* q;
-  int64_t q_stride;
-  int q_bf16;
-  int64_t n_tokens;
-  int hq, group;
-  const int32_t *starts, *contexts, *page_table;
-  int64_t table_stride;
-  int n_seqs;
-  int64_t max_new, max_context;
-  float scale_log2;
-  int causal, out_dtype;
-  void* out;
-  int* status;
-};
-
-// What the device arrays say of a sequence, cut to what the call allows.
-struct Span {
-  int64_t first, n;  // rows of q
-  int64_t ctx;
-};
-__device__ __forceinline__ Span span_of(const AttendArgs& a, int i) {
-  int64_t lo = a.starts[i], hi = a.starts[i + 1], ctx = a.contexts[i];
-  const int64_t room = min(a.max_context, a.table_stride << a.cache.page_shift);
-  bool bad = lo < 0 || hi < lo || hi > a.n_tokens || hi - lo > a.max_new || ctx < 0 || ctx > room;
-  lo = max((int64_t)0, min(lo, a.n_tokens));
-  hi = max(lo, min(min(hi, a.n_tokens), lo + a.max_new));
-  ctx = max((int64_t)0, min(ctx, room));
-  if (bad) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
-  return Span{lo, hi - lo, ctx};
-}
 
 // One warp per row: D / 32 elements a lane.
 template <int D>
@@ -50,11 +15,12 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
   constexpr int E = D / 32;
   const int lane = threadIdx.x & 31, seq = blockIdx.y;
   const Span sp = span_of(a, seq);
+  if (sp.n * a.group <= TOKEN_ROWS) return;
   const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
   if (row >= sp.n * a.hq) return;
   const int64_t t = row / a.hq;
   const int h = (int)(row % a.hq), kv = h / a.group;
-  const int64_t seen = a.causal ? max((int64_t)0, min(sp.ctx, sp.ctx - sp.n + t + 1)) : sp.ctx;
+  const int64_t seen = keys_seen(sp, t, a.causal);
   float q[E], o[E];
   const uint16_t* qp = a.q + (sp.first + t) * a.q_stride + h * D + lane * E;
 #pragma unroll
@@ -102,14 +68,33 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
   }
 }
 
+// The workspace: pieces of single tokens' rows, their maxima and sums.
+struct AttendWorkspace {
+  size_t off_ml = 0, bytes = 0;
+  int max_chunks = 1, part_rows = 0;
+};
+static AttendWorkspace attend_workspace(const turq_kv_cache* kc, int64_t n_tokens, int32_t n_seqs, int32_t n_q_heads, int64_t max_new,
+                                        int64_t max_context) {
+  AttendWorkspace w;
+  const int64_t group = n_q_heads / kc->n_kv_heads, most = max_new < n_tokens ? max_new : n_tokens;
+  if (group < 1 || group > TOKEN_ROWS) return w;
+  w.max_chunks = (int)token_chunks_max(max_context);
+  w.part_rows = (int)(most * group < TOKEN_ROWS ? most * group : TOKEN_ROWS);
+  if (w.max_chunks == 1) return w;
+  const size_t rows = (size_t)n_seqs * kc->n_kv_heads * w.max_chunks * w.part_rows;
+  w.off_ml = rows * kc->head_dim * 4;
+  w.bytes = w.off_ml + rows * 8;
+  return w;
+}
+
 }  // namespace turq
 
 extern "C" {
 
 size_t turq_kv_attention_workspace(const turq_kv_cache* cache, int64_t n_tokens, int32_t n_seqs, int32_t n_q_heads, int64_t max_new,
                                    int64_t max_context) {
-  (void)cache; (void)n_tokens; (void)n_seqs; (void)n_q_heads; (void)max_new; (void)max_context;
-  return 0;
+  if (!cache || n_tokens <= 0 || n_seqs <= 0 || n_q_heads <= 0 || max_new <= 0 || max_context <= 0) return 0;
+  return turq::attend_workspace(cache, n_tokens, n_seqs, n_q_heads, max_new, max_context).bytes;
 }
 
 int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void* dev_q, int64_t q_stride, int32_t q_dtype,
@@ -125,7 +110,7 @@ int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void*
   const int d = cache->head_dim, hkv = cache->n_kv_heads;
   if (n_q_heads < 1 || n_q_heads % hkv != 0 || n_q_heads / hkv > 128)
     return api_fail(ctx, TURQ_E_SHAPE, "n_q_heads must be a multiple of the cache's heads, at most 128 to one");
-  if (n_tokens < 0 || n_tokens > INT32_MAX / 2 || n_seqs < 0 || n_seqs > 65535) return api_fail(ctx, TURQ_E_SHAPE, "n_tokens or n_seqs out of range");
+  if (n_tokens < 0 || n_tokens > INT32_MAX / 2 || n_seqs < 0 || n_seqs > 65535 || hkv > 65535) return api_fail(ctx, TURQ_E_SHAPE, "n_tokens or n_seqs out of range");
   if (max_new < 0 || max_new > INT32_MAX / 2 || max_context < 0 || max_context > INT32_MAX / 2) return api_fail(ctx, TURQ_E_SHAPE, "max_new or max_context out of range");
   if (!(scale > 0.f) || scale > FLT_MAX) return api_fail(ctx, TURQ_E_INVALID_ARG, "scale must be positive and finite");
   if (n_tokens == 0 || n_seqs == 0 || max_new == 0) return TURQ_OK;
@@ -138,6 +123,7 @@ int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void*
   if ((uintptr_t)dev_starts % 4 != 0 || (uintptr_t)dev_contexts % 4 != 0 || (uintptr_t)dev_page_table % 4 != 0)
     return api_fail(ctx, TURQ_E_ALIGN, "starts, contexts and the page table must be 4-byte aligned");
   if (cache->device != ctx->device) return api_fail(ctx, TURQ_E_INVALID_ARG, "cache and context must live on the same device");
+  if (workspace_bytes > 0 && !dev_workspace) return api_fail(ctx, TURQ_E_INVALID_ARG, "null argument");
   if (workspace_bytes < turq_kv_attention_workspace(cache, n_tokens, n_seqs, n_q_heads, max_new, max_context))
     return api_fail(ctx, TURQ_E_SHAPE, "the workspace is smaller than turq_kv_attention_workspace");
   turq::AttendArgs a{};
@@ -162,13 +148,25 @@ int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void*
   a.status = ctx->dev_status;
   turq::DeviceScope on(ctx->device);
   if (on.status != cudaSuccess) return turq::api_cuda_fail(ctx, on.status, "attention launch");
-  const int64_t rows = (max_new < n_tokens ? max_new : n_tokens) * n_q_heads;
-  const dim3 grid((unsigned)((rows + 3) / 4), (unsigned)n_seqs);
-  if (d == 64) turq::attend_rows_kernel<64><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  else turq::attend_rows_kernel<128><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  const turq::AttendWorkspace w = turq::attend_workspace(cache, n_tokens, n_seqs, n_q_heads, max_new, max_context);
+  a.part = static_cast<float*>(dev_workspace);
+  a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(dev_workspace) + w.off_ml);
+  a.max_chunks = w.max_chunks;
+  a.part_rows = w.part_rows;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  const int64_t most = max_new < n_tokens ? max_new : n_tokens;
+  int launches = 0;
+  if (most * a.group > turq::TOKEN_ROWS) {
+    const dim3 grid((unsigned)((most * n_q_heads + 3) / 4), (unsigned)n_seqs);
+    if (d == 64) turq::attend_rows_kernel<64><<<grid, 128, 0, s>>>(a);
+    else turq::attend_rows_kernel<128><<<grid, 128, 0, s>>>(a);
+    e = cudaGetLastError();
+    launches++;
+  }
+  if (e == cudaSuccess && a.group <= turq::TOKEN_ROWS) e = turq::launch_attend_tokens(cache, a, s, &launches);
+  ctx->launches += launches;
   if (e != cudaSuccess) return turq::api_cuda_fail(ctx, e, "attention launch");
-  ctx->launches++;
   return TURQ_OK;
 }
 

@@ -1,0 +1,50 @@
+// What the kernels of attention over a paged cache share.
+#pragma once
+#include "../../include/turq.h"
+#include "attend_plan.h"
+#include "device_utils.cuh"
+#include "kvcache.cuh"
+
+namespace turq {
+
+struct AttendArgs {
+  KvPages cache;
+  const uint16_t* q;
+  int64_t q_stride;
+  int q_bf16;
+  int64_t n_tokens;
+  int hq, group;
+  const int32_t *starts, *contexts, *page_table;
+  int64_t table_stride;
+  int n_seqs;
+  int64_t max_new, max_context;
+  float scale_log2;  // scale x log2 e: weights are powers of two
+  int causal, out_dtype;
+  void* out;
+  int* status;
+  float *part, *part_ml;  // pieces of rows on their way to the kernel that joins them
+  int max_chunks, part_rows;
+};
+
+__device__ __forceinline__ void report(int* status, int code) { *reinterpret_cast<volatile int*>(status) = code; }
+
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int i) {
+  const Span s = cut_span(a.starts[i], a.starts[i + 1], a.contexts[i], a.n_tokens, a.max_new, a.max_context);
+  if (s.cut) report(a.status, TURQ_E_INVALID_ARG);
+  return s;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two neighbouring elements of the output, rounded once.
+__device__ __forceinline__ void store_out2(void* out, int dtype, int64_t i, float a, float b) {
+  if (dtype == TURQ_F32) *reinterpret_cast<float2*>(static_cast<float*>(out) + i) = make_float2(a, b);
+  else if (dtype == TURQ_BF16) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(out) + i) = __floats2bfloat162_rn(a, b);
+  else *reinterpret_cast<__half2*>(static_cast<__half*>(out) + i) = __floats2half2_rn(a, b);
+}
+
+}  // namespace turq

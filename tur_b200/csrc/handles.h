@@ -1,6 +1,7 @@
 // Definitions of the opaque handle types of the C ABI (shared by the translation units that
 // implement entry points).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -58,5 +59,8 @@ struct turq_kv_cache {
   int page_size = 0, n_kv_heads = 0, head_dim = 0;
   uint8_t* mem = nullptr;
   bool owns = false;
-  size_t off_k = 0, off_v = 0, off_ks = 0, off_vs = 0, bytes = 0;
+  size_t off_v = 0, off_ks = 0, off_vs = 0, bytes = 0;
+  // The planes for copies by the tensor memory accelerator: boxes of 16 tokens of a page (one 128-byte column block of the
+  // 16-bit types, a whole row of int8) and the scales of 16 tokens. What lies outside the planes reads as zeros.
+  CUtensorMap k16, v16, ks16, vs16;
 };

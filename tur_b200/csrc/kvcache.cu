@@ -297,6 +297,46 @@ int32_t run_head_rows(turq_ctx* ctx, int head_dim, const turq::HeadRowsArgs& a, 
   return TURQ_OK;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A plane [n_pages * heads][page_size][row_elems] for boxes of `tokens` rows and `cols` elements.
+bool map_plane(EncodeTiledFn enc, CUtensorMap* map, const turq_kv_cache* kc, CUtensorMapDataType type, int elem, size_t offset, int row_elems,
+               int cols, int tokens, CUtensorMapSwizzle swizzle) {
+  const cuuint64_t dims[3] = {(cuuint64_t)row_elems, (cuuint64_t)kc->page_size, (cuuint64_t)kc->n_pages * kc->n_kv_heads};
+  const cuuint64_t strides[2] = {(cuuint64_t)row_elems * elem, (cuuint64_t)row_elems * elem * kc->page_size};
+  const cuuint32_t box[3] = {(cuuint32_t)cols, (cuuint32_t)tokens, 1}, step[3] = {1, 1, 1};
+  return enc(map, type, 3, kc->mem + offset, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool map_planes(turq_kv_cache* kc) {
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return false;
+  const EncodeTiledFn enc = reinterpret_cast<EncodeTiledFn>(p);
+  const int d = kc->head_dim;
+  if (kc->dtype != TURQ_Q8_0) {
+    const CUtensorMapDataType t = kc->dtype == TURQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return map_plane(enc, &kc->k16, kc, t, 2, 0, d, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           map_plane(enc, &kc->v16, kc, t, 2, kc->off_v, d, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  // Rows of 64 bytes are read without conflicts as they lie. Scales: the 16 tokens' lie one behind the other, so a page
+  // is one row of its head's plane.
+  const CUtensorMapSwizzle swizzle = d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE;
+  const int per = d / 32;
+  auto scales = [&](CUtensorMap* map, size_t offset) {
+    const cuuint64_t dims[2] = {(cuuint64_t)kc->page_size * per, (cuuint64_t)kc->n_pages * kc->n_kv_heads};
+    const cuuint64_t strides[1] = {(cuuint64_t)kc->page_size * per * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)(16 * per), 1}, step[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, kc->mem + offset, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  return map_plane(enc, &kc->k16, kc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 0, d, d, 16, swizzle) &&
+         map_plane(enc, &kc->v16, kc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kc->off_v, d, d, 16, swizzle) && scales(&kc->ks16, kc->off_ks) &&
+         scales(&kc->vs16, kc->off_vs);
+}
+
 struct CacheShape { size_t off_v, off_ks, off_vs, bytes; bool ok; };
 CacheShape cache_shape(int32_t dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim) {
   CacheShape c{0, 0, 0, 0, false};
@@ -406,6 +446,10 @@ int32_t turq_kv_cache_create(turq_ctx* ctx, int32_t dtype, int64_t n_pages, int3
       turq_kv_cache_free(kc);
       return api_cuda_fail(ctx, e, "allocating the cache's pages");
     }
+  }
+  if (!map_planes(kc)) {
+    turq_kv_cache_free(kc);
+    return api_fail(ctx, TURQ_E_CUDA, "the driver does not describe the cache's pages as tensors");
   }
   *out = kc;
   return TURQ_OK;
