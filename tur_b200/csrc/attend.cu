@@ -1,6 +1,8 @@
 // Attention of new tokens over a paged cache (src/models/qwen3.rs:308-505; src/models/attention/cpu_flash).
 // out[t, h] = sum_j p_j V_j / sum_j p_j with p_j = exp(scale q . K_j - m), one pass over the keys with the
-// running maximum m and sum.
+// running maximum m and sum. The entry and the choice between the kernels: up to TOKEN_ROWS rows (new tokens x query
+// heads) per key head of a sequence go to attend_tokens.cu, more to attend_tiles.cu. A call may hold both; the lengths
+// are on the device, so both are launched and each takes its own.
 #include <cfloat>
 
 #include "attend.cuh"
@@ -8,65 +10,6 @@
 #include "turq_internal.h"
 
 namespace turq {
-
-// One warp per row: D / 32 elements a lane.
-template <int D>
-__global__ void __launch_bounds__(128) attend_rows_kernel(const AttendArgs a) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31, seq = blockIdx.y;
-  const Span sp = span_of(a, seq);
-  if (sp.n * a.group <= TOKEN_ROWS) return;
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  if (row >= sp.n * a.hq) return;
-  const int64_t t = row / a.hq;
-  const int h = (int)(row % a.hq), kv = h / a.group;
-  const int64_t seen = keys_seen(sp, t, a.causal);
-  float q[E], o[E];
-  const uint16_t* qp = a.q + (sp.first + t) * a.q_stride + h * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    q[e] = a.q_bf16 ? __uint_as_float((uint32_t)qp[e] << 16) : f16_bits_to_f32(qp[e]);
-    o[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = 0; j < seen; j++) {
-    const int32_t page = a.page_table[seq * a.table_stride + (j >> a.cache.page_shift)];
-    const bool known = page >= 0 && page < a.cache.n_pages;
-    if (!known) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
-    const int64_t at = a.cache.row(((int64_t)(known ? page : 0) << a.cache.page_shift) + (j & (a.cache.page_size - 1)), kv);
-    float k[E], v[E], s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int64_t i = at * D + lane * E + e;
-      if (a.cache.dtype == TURQ_Q8_0) {
-        k[e] = (float)reinterpret_cast<const int8_t*>(a.cache.k)[i] * __half2float(a.cache.ks[i / 32]);
-        v[e] = (float)reinterpret_cast<const int8_t*>(a.cache.v)[i] * __half2float(a.cache.vs[i / 32]);
-      } else {
-        const uint16_t kb = reinterpret_cast<const uint16_t*>(a.cache.k)[i], vb = reinterpret_cast<const uint16_t*>(a.cache.v)[i];
-        k[e] = a.cache.dtype == TURQ_BF16 ? __uint_as_float((uint32_t)kb << 16) : f16_bits_to_f32(kb);
-        v[e] = a.cache.dtype == TURQ_BF16 ? __uint_as_float((uint32_t)vb << 16) : f16_bits_to_f32(vb);
-      }
-      if (!known) k[e] = v[e] = 0.f;
-      s += q[e] * k[e];
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-    s *= a.scale_log2;
-    const float m2 = fmaxf(m, s), was = m2 == -INFINITY ? 0.f : exp2f(m - m2), p = m2 == -INFINITY ? 0.f : exp2f(s - m2);
-    l = l * was + p;
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = o[e] * was + p * v[e];
-    m = m2;
-  }
-  const int64_t out = ((sp.first + t) * a.hq + h) * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const float y = l > 0.f ? o[e] / l : 0.f;
-    if (a.out_dtype == TURQ_F32) static_cast<float*>(a.out)[out + e] = y;
-    else if (a.out_dtype == TURQ_BF16) static_cast<__nv_bfloat16*>(a.out)[out + e] = __float2bfloat16_rn(y);
-    else static_cast<__half*>(a.out)[out + e] = __float2half_rn(y);
-  }
-}
 
 // The workspace: pieces of single tokens' rows, their maxima and sums.
 struct AttendWorkspace {
@@ -158,11 +101,10 @@ int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void*
   const int64_t most = max_new < n_tokens ? max_new : n_tokens;
   int launches = 0;
   if (most * a.group > turq::TOKEN_ROWS) {
-    const dim3 grid((unsigned)((most * n_q_heads + 3) / 4), (unsigned)n_seqs);
-    if (d == 64) turq::attend_rows_kernel<64><<<grid, 128, 0, s>>>(a);
-    else turq::attend_rows_kernel<128><<<grid, 128, 0, s>>>(a);
-    e = cudaGetLastError();
-    launches++;
+    const int64_t per_tile = 2 * (128 / a.group);  // tokens
+    const int64_t tiles = n_tokens / per_tile + n_seqs;  // no fewer than there are
+    if (tiles * hkv > INT32_MAX) return api_fail(ctx, TURQ_E_LIMIT, "more row tiles than a launch takes");
+    e = turq::launch_attend_tiles(cache, a, tiles, 1, s, &launches);
   }
   if (e == cudaSuccess && a.group <= turq::TOKEN_ROWS) e = turq::launch_attend_tokens(cache, a, s, &launches);
   ctx->launches += launches;

@@ -1,0 +1,562 @@
+// Attention of many rows over a paged cache (chunks, prompts) on the 5th-generation tensor cores.
+//
+// A CTA takes two tiles of up to 128 rows (row = new token x query head of one key head, heads of a token side by
+// side, so all rows share K and V) and walks the keys in tiles of 128:
+//   * warp 9        copies K and V tiles page by page by TMA into a ring (and prefetches the page table), and zeroes the
+//                   values behind the context's end (they may be anything, and 0 x NaN is NaN);
+//   * warps 12..15  Q8_0 only: int8 tiles and their scales -> f16 operand tiles;
+//   * warp 8        one lane issues tcgen05.mma: S_t = Q_t K^T (both from shared memory), O_t += P_t V (P from TMEM);
+//   * warps 0..3 and 4..7  softmax of tile 0 and of tile 1, a thread per row: S from TMEM, running maximum and sum in
+//                   registers, P back into S's columns, and the division at the end. The two tiles take turns: while
+//                   the tensor core works on one the other's weights are computed.
+// O is rescaled only where a row's maximum grew by more than 2^8 (weights and their sum then stay within f16 and
+// f32, and the quotient is the same); a thread owns its row, so that costs the warp that needs it 2 x D columns of TMEM.
+// Rows to TMEM lanes: softmax thread r of a tile is lane r. Order of the MMAs: PV of a tile is issued before the
+// next S of that tile, whose columns hold P, and a commit covers all MMAs before it: a full S says that O is complete.
+#include "attend.cuh"
+#include "attend_launch.h"
+#include "tc_common.cuh"
+#include "turq_internal.h"
+
+namespace turq {
+
+constexpr int TILE_M = 128, TILE_N = 128;
+
+template <int D, bool Q8> struct TileGeomA {
+  static constexpr int HALVES = D / 64;
+  static constexpr int OPERAND = TILE_N * D * 2;      // a tile of K, V or Q: blocks of 64 columns, 128 rows of 128 bytes each
+  static constexpr int STAGES = Q8 ? 3 : (D == 128 ? 5 : 8);
+  static constexpr int RAW = Q8 ? TILE_N * D + 1024 : 0;  // int8 rows, scales behind them
+  static constexpr int RAW_STAGES = Q8 ? 3 : 0;
+  static constexpr int THREADS = Q8 ? 512 : 384;
+  static constexpr int REG_SOFT = Q8 ? 192 : 208, REG_REST = Q8 ? 64 : 88;
+  static constexpr int SMEM = 2 * OPERAND + STAGES * OPERAND + RAW_STAGES * RAW + 1024;
+  static_assert(256 * REG_SOFT + (THREADS - 256) * REG_REST <= THREADS * (Q8 ? 128 : 168), "registers of the launch");
+};
+
+__device__ __forceinline__ void tmem_ld32(float* v, uint32_t addr) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+        "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld16(float* v, uint32_t addr) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+               "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(da), "l"(db),
+               "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db),
+               "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void tile_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tile_box2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack_p(float a, float b) {
+  if (BF) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+  const __half2 t = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// Bounded: after an expiry the abort flag ends every further wait, and what a loop then does stays within its buffers.
+// (In line: a call would not fit the uneven split of registers.)
+__device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (!bar_try(bar, parity)) {
+    const long long t0 = clock64();
+    while (!bar_try(bar, parity)) {
+      if (*abort_flag || clock64() - t0 > TC_WAIT_CYCLES) {
+        *abort_flag = 1;
+        break;
+      }
+    }
+  }
+  __syncwarp();  // what follows is done by the warp as one
+}
+
+struct TileMaps { CUtensorMap k, v, ks, vs; };
+
+struct Work {
+  Span sp;
+  int seq, head, tok0, live;     // first new token of the CTA; whether there is any work
+  int id;                        // (list index x heads + head), for pieces
+  int begin, end;                // key tiles
+};
+
+// The blockIdx.x / heads-th tile of the call, a sequence's last (longest) first.
+__device__ __forceinline__ void find_work(const AttendArgs& a, int tokens_per_cta, int splits, Work* w, int lane) {
+  int want = (int)(blockIdx.x / a.cache.n_heads);
+  const int head = (int)(blockIdx.x % a.cache.n_heads);
+  if (lane == 0) w->live = 0;
+  __syncwarp();
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+    Span sp{};
+    int tiles = 0;
+    if (s0 + lane < a.n_seqs) {
+      sp = span_of(a, s0 + lane);
+      if (sp.n * a.group > TOKEN_ROWS) tiles = (int)((sp.n + tokens_per_cta - 1) / tokens_per_cta);
+    }
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int t = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+      if (lane >= d) upto += t;
+    }
+    const int total = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (want < total) {
+      if (want < upto && want >= upto - tiles) {
+        const int tile = tiles - 1 - (want - (upto - tiles));
+        w->sp = sp;
+        w->seq = s0 + lane;
+        w->head = head;
+        w->tok0 = tile * tokens_per_cta;
+        w->id = (int)blockIdx.x;
+        const int64_t last = min(sp.n, (int64_t)w->tok0 + tokens_per_cta) - 1;
+        const int keys = (int)min(sp.ctx, keys_seen(sp, last, a.causal));
+        const int n = (keys + TILE_N - 1) / TILE_N;
+        w->begin = (int)((int64_t)n * blockIdx.y / splits);
+        w->end = (int)((int64_t)n * (blockIdx.y + 1) / splits);
+        w->live = 1;
+      }
+      break;
+    }
+    want -= total;
+  }
+  __syncwarp();
+}
+
+template <int D, bool Q8, bool BF>
+__global__ void __launch_bounds__((TileGeomA<D, Q8>::THREADS), 1)
+attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ AttendArgs a) {
+  using G = TileGeomA<D, Q8>;
+  constexpr int ST = G::STAGES, OP = G::OPERAND, HB = TILE_N * 128;  // HB: one 64-column block
+  constexpr uint32_t COL_S = 0, COL_O = 256;                          // S (and P) of tile t at 128 t, O at 256 + D t
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full, v_fixed, raw_full[3], raw_empty[3];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ Work work;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem = (s_u32(raw) + 1023u) & ~1023u;
+  const uint32_t sQ = smem, sKV = smem + 2 * OP, sRaw = sKV + ST * OP;
+  volatile int* const abort_flag = &abort_word;
+  const int tpt = TILE_M / a.group;  // tokens of a tile
+
+  if (warp == 0) find_work(a, 2 * tpt, (int)gridDim.y, &work, lane);
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < 2; i++) { bar_init(&q_full[i], 4); bar_init(&s_full[i], 1); bar_init(&p_full[i], 4); }
+    for (int i = 0; i < ST; i++) { bar_init(&kv_full[i], Q8 ? 4 : 1); bar_init(&kv_empty[i], 1); }
+    bar_init(&o_full, 1);
+    bar_init(&v_fixed, 1);
+    for (int i = 0; i < 3; i++) { bar_init(&raw_full[i], 1); bar_init(&raw_empty[i], 4); }
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (!work.live) return;
+  const Span sp = work.sp;
+  const int seq = work.seq, head = work.head, begin = work.begin, n_iter = work.end - work.begin;
+  const int tiles = sp.n - work.tok0 > tpt ? 2 : 1;  // row tiles with rows
+  const int ctx = (int)sp.ctx;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&tmem_slot)), "n"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::REG_SOFT));
+    const int t = warp >> 2, r = threadIdx.x & 127;
+    const int tok = work.tok0 + t * tpt + r / a.group;
+    const bool live = r < tpt * a.group && tok < sp.n;
+    const int qh = head * a.group + r % a.group;
+    float mul = a.scale_log2;
+    // Q into the operand layout; on f16 caches a bf16 row by the power of two that its largest element fits
+    if (t < tiles) {
+      const uint4* qp = reinterpret_cast<const uint4*>(a.q + (sp.first + (live ? tok : 0)) * a.q_stride + (int64_t)qh * D);
+      const bool convert = !BF && a.q_bf16;
+      float down = 1.f;
+      if (convert) {
+        uint32_t top = 0;
+        for (int i = 0; i < D / 8; i++) {
+          const uint4 w = live ? qp[i] : make_uint4(0, 0, 0, 0);
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) top = max(top, max(x[e] & 0x7FFFu, (x[e] >> 16) & 0x7FFFu));
+        }
+        const int e = min(max((int)(top >> 7) - 127, -100), 100);
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
+        mul *= __uint_as_float((uint32_t)(127 + e) << 23);
+      }
+#pragma unroll 4
+      for (int i = 0; i < D / 8; i++) {
+        uint4 w = live ? qp[i] : make_uint4(0, 0, 0, 0);
+        if (convert) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = pack_p<false>(__uint_as_float(x[e] << 16) * down, __uint_as_float(x[e] & 0xFFFF0000u) * down);
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sQ + t * OP + (i >> 3) * HB + r * 128 + (((i & 7) ^ (r & 7)) << 4)), "r"(w.x), "r"(w.y),
+                     "r"(w.z), "r"(w.w) : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(&q_full[t]);
+    }
+    const int seen = live ? (int)min(sp.ctx, keys_seen(sp, tok, a.causal)) : INT32_MAX;  // rows that do not exist ask for no mask
+    // keys that every row of the warp sees
+    int least = seen;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, d));
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in the address' upper half
+    const uint32_t tS = tmem + lanes + COL_S + 128 * t, tO = tmem + lanes + COL_O + D * t;
+    float m = -INFINITY, l = 0.f;  // maximum in units of S, as last subtracted; sum of the weights
+    const float lag = 8.f / mul;
+    if (t < tiles) {
+      for (int j = 0; j < n_iter; j++) {
+        float s[TILE_N];
+        tile_wait(&s_full[t], j & 1, abort_flag);
+        tc_after();
+#pragma unroll
+        for (int i = 0; i < 4; i++) tmem_ld32(s + 32 * i, tS + 32 * i);
+        tmem_wait_ld();
+        const int k0 = (begin + j) * TILE_N;
+        if (k0 + TILE_N > least) {
+          const int lim = seen - k0;
+#pragma unroll
+          for (int i = 0; i < TILE_N; i++) s[i] = i < lim ? s[i] : -INFINITY;
+        }
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < TILE_N; i += 4) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], s[i + e]);
+        }
+        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (j == 0) {
+          m = mt;
+        } else if (__any_sync(0xFFFFFFFFu, mt > m + lag)) {
+          const float m2 = fmaxf(m, mt), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * mul);  // m = -inf: 0 of nothing
+          m = m2;
+          l *= f;
+          float o[16];
+#pragma unroll 1
+          for (int i = 0; i < D / 16; i++) {
+            tmem_ld16(o, tO + 16 * i);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[e] *= f;
+            tmem_st16(tO + 16 * i, reinterpret_cast<const uint32_t*>(o));
+          }
+          tmem_wait_st();
+        }
+        const float sub = m == -INFINITY ? 0.f : m * mul;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < TILE_N / 32; h++) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float x = ex2(fmaf(s[32 * h + 2 * i], mul, -sub)), y = ex2(fmaf(s[32 * h + 2 * i + 1], mul, -sub));
+            sum[(2 * i) & 3] += x;
+            sum[(2 * i + 1) & 3] += y;
+            p[i] = pack_p<BF>(x, y);
+          }
+          tmem_st16(tS + 16 * h, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&p_full[t]);
+      }
+      if (n_iter > 0) {
+        tile_wait(&o_full, 0, abort_flag);
+        tc_after();
+      }
+      const bool pieces = gridDim.y > 1;
+      const float inv = pieces ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a row that sees no key gives zeros; NaN stays
+      const int64_t out = ((sp.first + tok) * a.hq + qh) * D;
+      const int64_t piece = ((int64_t)work.id * gridDim.y + blockIdx.y) * (2 * TILE_M) + TILE_M * t + r;
+      if (pieces) *reinterpret_cast<float2*>(a.part_ml + 2 * piece) = make_float2(m * mul, live ? l : 0.f);
+      const bool store = live && !*abort_flag;
+      for (int i = 0; i < D / 32; i++) {
+        float o[32];
+        __syncwarp();
+        if (n_iter > 0) {
+          tmem_ld32(o, tO + 32 * i);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] = 0.f;
+        }
+        if (!store) {
+        } else if (pieces) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(a.part + piece * D + 32 * i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else if (a.out_dtype == TURQ_F32) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + out + 32 * i + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+        } else {
+          const bool bf = a.out_dtype == TURQ_BF16;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+              const float x = o[e + 2 * q] * inv, y = o[e + 2 * q + 1] * inv;
+              w[q] = bf ? pack_p<true>(x, y) : pack_p<false>(x, y);
+            }
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + out + 32 * i + e) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::REG_REST));
+    if (warp == 8) {
+      // -------------------------------------------------------------- MMA
+      constexpr uint32_t type = BF ? (1u << 7) | (1u << 10) : 0u;
+      constexpr uint32_t id_qk = (1u << 4) | type | ((TILE_N >> 3) << 17) | ((TILE_M >> 4) << 24);
+      constexpr uint32_t id_pv = (1u << 4) | type | (1u << 16) | ((D >> 3) << 17) | ((TILE_M >> 4) << 24);  // V: the columns lie side by side
+      // rows of 128 swizzled bytes, eight of them 1024 bytes apart; for V also the step from one block of 64 columns to the next
+      constexpr uint64_t k_hi = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+      constexpr uint64_t v_hi = ((uint64_t)(HB >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+      const uint32_t q_lo = (sQ & 0x3FFFFu) >> 4, kv_lo = (sKV & 0x3FFFFu) >> 4;
+      const bool issuer = elect_one();
+      auto qk = [&](int t, int stage) {
+        if (!issuer) return;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) {
+          const uint32_t off = (uint32_t)((i >> 2) * (HB >> 4) + 2 * (i & 3));
+          mma_ss(tmem + COL_S + 128 * t, k_hi | (uint64_t)(q_lo + t * (OP >> 4) + off), k_hi | (uint64_t)(kv_lo + stage * (OP >> 4) + off), id_qk, i > 0);
+        }
+        tc_commit(&s_full[t]);
+      };
+      auto pv = [&](int t, int stage, bool first) {
+        if (!issuer) return;
+#pragma unroll
+        for (int i = 0; i < TILE_N / 16; i++)
+          mma_ts(tmem + COL_O + D * t, tmem + COL_S + 128 * t + 8 * i, v_hi | (uint64_t)(kv_lo + stage * (OP >> 4) + 128 * i), id_pv, !first || i > 0);
+      };
+      if (n_iter > 0) {
+        int ks = 0, vs = 1 % ST;  // stages: K_0, V_0, K_1, V_1, ...
+        uint32_t kp = 0, vp = 1 >= ST;
+        auto next = [](int& s, uint32_t& p) {
+          s += 2;
+          if (s >= ST) { s -= ST; p ^= 1u; }
+        };
+        for (int t = 0; t < tiles; t++) tile_wait(&q_full[t], 0, abort_flag);
+        tile_wait(&kv_full[ks], kp, abort_flag);
+        tc_after();
+        for (int t = 0; t < tiles; t++) qk(t, ks);
+        if (issuer) tc_commit(&kv_empty[ks]);
+        next(ks, kp);
+        for (int j = 0; j < n_iter; j++) {
+          if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
+          const bool more = j + 1 < n_iter;
+          tile_wait(&kv_full[vs], vp, abort_flag);
+          if (!Q8 && (begin + j + 1) * TILE_N > ctx) tile_wait(&v_fixed, 0, abort_flag);
+          for (int t = 0; t < tiles; t++) {
+            tile_wait(&p_full[t], j & 1, abort_flag);
+            tc_after();
+            pv(t, vs, j == 0);
+            if (t == tiles - 1 && issuer) tc_commit(&kv_empty[vs]);
+            if (more) {
+              if (t == 0) {
+                tile_wait(&kv_full[ks], kp, abort_flag);
+                tc_after();
+              }
+              qk(t, ks);
+              if (t == tiles - 1 && issuer) tc_commit(&kv_empty[ks]);
+            }
+          }
+          next(vs, vp);
+          next(ks, kp);
+        }
+        if (issuer) tc_commit(&o_full);
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // -------------------------------------------------------------- copies
+      // lane i: the page that key 16 i of the tile begins (boxes of a page's tokens, 16 to 128 of them)
+      const int box = min(a.cache.page_size, TILE_N), boxes = TILE_N / box;
+      const int32_t* table = a.page_table + seq * a.table_stride;
+      auto page_of = [&](int j) {  // z coordinate of this lane's box in key tile begin + j; -1: behind the context
+        const int64_t key = (int64_t)(begin + j) * TILE_N + lane * box;
+        if (lane >= boxes || j >= n_iter || key >= ctx) return -1;
+        const int64_t p = table[key >> a.cache.page_shift];
+        const bool known = p >= 0 && p < a.cache.n_pages;
+        if (!known) report(a.status, TURQ_E_INVALID_ARG);
+        return known ? (int)(p * a.cache.n_heads + head) : (int)(a.cache.n_pages * a.cache.n_heads);
+      };
+      int stage = 0, z = page_of(0);
+      uint32_t ph = 0;
+      for (int j = 0; j < n_iter; j++) {
+        if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
+        const int z2 = page_of(j + 1);
+        const int y = ((begin + j) * TILE_N + lane * box) & (a.cache.page_size - 1);
+        const int n = __popc(__ballot_sync(0xFFFFFFFFu, z >= 0));
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+          if (!Q8) {
+            tile_wait(&kv_empty[stage], ph ^ 1u, abort_flag);
+            const uint32_t bar = s_u32(&kv_full[stage]), at = sKV + stage * OP + lane * box * 128;
+            if (lane == 0) bar_expect_tx(&kv_full[stage], n * box * D * 2);
+            __syncwarp();
+            if (z >= 0) {
+#pragma unroll
+              for (int h = 0; h < G::HALVES; h++) tile_box3(at + h * HB, kv ? &maps.v : &maps.k, 64 * h, y, z, bar);
+            }
+            if (++stage == ST) { stage = 0; ph ^= 1u; }
+          } else {
+            tile_wait(&raw_empty[stage], ph ^ 1u, abort_flag);
+            const uint32_t bar = s_u32(&raw_full[stage]), at = sRaw + stage * G::RAW;
+            if (lane == 0) bar_expect_tx(&raw_full[stage], n * box * (D + D / 16));
+            __syncwarp();
+            if (z >= 0) {
+              tile_box3(at + lane * box * D, kv ? &maps.v : &maps.k, 0, y, z, bar);
+              // scales: 16 keys' in 128 bytes each (of which D = 64 fills half), as copies ask for
+              for (int b = 0; b < box / 16; b++)
+                tile_box2(at + TILE_N * D + (lane * box / 16 + b) * 128, kv ? &maps.vs : &maps.ks, (y + 16 * b) * (D / 32), z, bar);
+            }
+            if (++stage == G::RAW_STAGES) { stage = 0; ph ^= 1u; }
+          }
+        }
+        z = z2;
+      }
+      // Values behind the context's end. Only this warp can wait for a phase of kv_full that is many on: it knows that the one
+      // before is over, as its own wait for the empty stage said.
+      if (!Q8 && n_iter > 0 && (begin + n_iter) * TILE_N > ctx) {
+        const int i = 2 * (n_iter - 1) + 1, last = i % ST, from = ctx - (begin + n_iter - 1) * TILE_N;
+        tile_wait(&kv_full[last], (i / ST) & 1, abort_flag);
+        for (int c = lane; c < (TILE_N - from) * (D / 8); c += 32) {
+          const int row = from + c / (D / 8), ch = c % (D / 8);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(sKV + last * OP + (ch >> 3) * HB + row * 128 + ((ch & 7) << 4)), "r"(0u) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(&v_fixed);
+      }
+    } else if (warp >= 12) {
+      // -------------------------------------------------------------- int8 -> f16 operand tiles
+      const int id0 = threadIdx.x - 384;
+      int rs = 0, stage = 0;
+      uint32_t rp = 0, ph = 0;
+      for (int j = 0; j < 2 * n_iter; j++) {
+        const int keys = ctx - (begin + (j >> 1)) * TILE_N;  // that exist, of this tile
+        tile_wait(&raw_full[rs], rp, abort_flag);
+        tile_wait(&kv_empty[stage], ph ^ 1u, abort_flag);
+        const uint32_t src = sRaw + rs * G::RAW, dst = sKV + stage * OP;
+#pragma unroll 4
+        for (int i = 0; i < D / 16; i++) {
+          const int id = i * 128 + id0, row = id / (D / 16), ch = id % (D / 16);
+          uint4 w;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(src + id * 16));
+          uint16_t sc;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc) : "r"(src + TILE_N * D + (row >> 4) * 128 + ((row & 15) * (D / 32) + (ch >> 1)) * 2));
+          const __half2 scale = __half2half2(__ushort_as_half(sc)), off = __float2half2_rn(1152.f);
+          const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            h[2 * e] = h22u(__hmul2(__hsub2(pair01(x[e]), off), scale));
+            h[2 * e + 1] = h22u(__hmul2(__hsub2(pair23(x[e]), off), scale));
+          }
+          if (row >= keys) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) h[e] = 0u;
+          }
+          const uint32_t to = dst + (ch >> 2) * HB + row * 128;
+          const int c0 = ((2 * ch) & 7) ^ (row & 7), c1 = ((2 * ch + 1) & 7) ^ (row & 7);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + (c0 << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + (c1 << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          bar_arrive(&kv_full[stage]);
+          bar_arrive(&raw_empty[rs]);
+        }
+        if (++rs == G::RAW_STAGES) { rs = 0; rp ^= 1u; }
+        if (++stage == ST) { stage = 0; ph ^= 1u; }
+      }
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // a wait ran out: give copies still in flight time to land in this CTA's shared memory
+    for (int i = 0; i < 64; i++) __nanosleep(2000);
+    if (threadIdx.x == 0) report(a.status, TURQ_E_TIMEOUT);
+  }
+  if (warp == 8) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+  }
+}
+
+template <int D, bool Q8, bool BF>
+static cudaError_t launch_tiles(const turq_kv_cache* kc, const AttendArgs& a, int64_t tiles, int splits, cudaStream_t s) {
+  using G = TileGeomA<D, Q8>;
+  static PerDeviceOnce configured;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!configured.done(dev)) {
+    e = cudaFuncSetAttribute(attend_tiles_kernel<D, Q8, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+    if (e != cudaSuccess) return e;
+    configured.set(dev);
+  }
+  const TileMaps maps{kc->k_tile, kc->v_tile, kc->ks16, kc->vs16};
+  attend_tiles_kernel<D, Q8, BF><<<dim3((unsigned)(tiles * a.cache.n_heads), (unsigned)splits), G::THREADS, G::SMEM, s>>>(maps, a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_attend_tiles(const turq_kv_cache* kc, const AttendArgs& a, int64_t tiles, int splits, cudaStream_t s, int* launches) {
+  (*launches)++;
+  if (kc->head_dim == 128) {
+    if (kc->dtype == TURQ_Q8_0) return launch_tiles<128, true, false>(kc, a, tiles, splits, s);
+    return kc->dtype == TURQ_BF16 ? launch_tiles<128, false, true>(kc, a, tiles, splits, s) : launch_tiles<128, false, false>(kc, a, tiles, splits, s);
+  }
+  if (kc->dtype == TURQ_Q8_0) return launch_tiles<64, true, false>(kc, a, tiles, splits, s);
+  return kc->dtype == TURQ_BF16 ? launch_tiles<64, false, true>(kc, a, tiles, splits, s) : launch_tiles<64, false, false>(kc, a, tiles, splits, s);
+}
+
+}  // namespace turq

@@ -63,4 +63,5 @@ struct turq_kv_cache {
   // The planes for copies by the tensor memory accelerator: boxes of 16 tokens of a page (one 128-byte column block of the
   // 16-bit types, a whole row of int8) and the scales of 16 tokens. What lies outside the planes reads as zeros.
   CUtensorMap k16, v16, ks16, vs16;
+  CUtensorMap k_tile, v_tile;  // boxes of a whole page, or of 128 of its tokens
 };

@@ -315,11 +315,13 @@ bool map_planes(turq_kv_cache* kc) {
   cudaDriverEntryPointQueryResult q;
   if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return false;
   const EncodeTiledFn enc = reinterpret_cast<EncodeTiledFn>(p);
-  const int d = kc->head_dim;
+  const int d = kc->head_dim, whole = kc->page_size < 128 ? kc->page_size : 128;
   if (kc->dtype != TURQ_Q8_0) {
     const CUtensorMapDataType t = kc->dtype == TURQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     return map_plane(enc, &kc->k16, kc, t, 2, 0, d, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B) &&
-           map_plane(enc, &kc->v16, kc, t, 2, kc->off_v, d, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B);
+           map_plane(enc, &kc->v16, kc, t, 2, kc->off_v, d, 64, 16, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           map_plane(enc, &kc->k_tile, kc, t, 2, 0, d, 64, whole, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           map_plane(enc, &kc->v_tile, kc, t, 2, kc->off_v, d, 64, whole, CU_TENSOR_MAP_SWIZZLE_128B);
   }
   // Rows of 64 bytes are read without conflicts as they lie. Scales: the 16 tokens' lie one behind the other, so a page
   // is one row of its head's plane.
@@ -333,7 +335,9 @@ bool map_planes(turq_kv_cache* kc) {
                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
   return map_plane(enc, &kc->k16, kc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 0, d, d, 16, swizzle) &&
-         map_plane(enc, &kc->v16, kc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kc->off_v, d, d, 16, swizzle) && scales(&kc->ks16, kc->off_ks) &&
+         map_plane(enc, &kc->v16, kc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kc->off_v, d, d, 16, swizzle) &&
+         map_plane(enc, &kc->k_tile, kc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 0, d, d, whole, CU_TENSOR_MAP_SWIZZLE_NONE) &&
+         map_plane(enc, &kc->v_tile, kc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kc->off_v, d, d, whole, CU_TENSOR_MAP_SWIZZLE_NONE) && scales(&kc->ks16, kc->off_ks) &&
          scales(&kc->vs16, kc->off_vs);
 }
 
