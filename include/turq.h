@@ -343,8 +343,9 @@ int32_t turq_kv_read(turq_ctx* ctx, const turq_kv_cache* cache, const int64_t* d
  * turq_ctx_poll_status reports it. dev_workspace holds turq_kv_attention_workspace bytes (which may
  * be 0) with the same bounds; it needs no initial value, and is the call's own until it has
  * run: two calls that may overlap need two.
- * For up to 16 rows per key head (new tokens x query heads to one) a row's bits do not depend on
- * the other sequences of the call; for more, how a long context is cut goes by the whole call. */
+ * The same call gives the same bits; how long contexts are cut into pieces, whose f32 sums are then
+ * added in order, goes by n_seqs, max_new and max_context, so between calls of other bounds a
+ * row's last bits may differ. */
 size_t turq_kv_attention_workspace(const turq_kv_cache* cache, int64_t n_tokens, int32_t n_seqs, int32_t n_q_heads, int64_t max_new,
                                    int64_t max_context);
 int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void* dev_q, int64_t q_stride, int32_t q_dtype,

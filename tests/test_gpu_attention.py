@@ -359,17 +359,19 @@ def test_rows_outside_the_sequences_stay_and_strides_are_taken():
     tq.context().poll_status()
 
 
-def test_a_tokens_bits_do_not_depend_on_the_other_sequences():
-    spans = [(1, 1234), (1, 5000), (2, 300), (1, 17), (4, 2600)]
+def test_the_same_call_gives_the_same_bits():
+    """Also for a sequence whose neighbours' keys, queries and lengths change within the call's bounds."""
+    spans = [(1, 1234), (1, 5000), (2, 300), (1, 17), (200, 2600), (1, 5000)]
     for kind in (torch.bfloat16, "q8_0"):
         cache, table, q, starts, contexts, k, v = make_case(12, spans, kind, torch.bfloat16, 8, 2, 128, 16)
-        whole = cache.attend(q, starts, contexts, table, max_new=4)
-        for i, (new, ctx) in enumerate(spans):
-            a = int(starts[i])
-            one = torch.tensor([0, new], dtype=torch.int32, device="cuda")
-            alone = cache.attend(q[a:a + new].contiguous(), one, contexts[i:i + 1].contiguous(), table[i:i + 1].contiguous())
-            assert torch.equal(alone, whole[a:a + new])
-        assert torch.equal(cache.attend(q, starts, contexts, table), cache.attend(q, starts, contexts, table))
+        bounds = {"max_new": 200, "max_context": 5000}
+        whole = cache.attend(q, starts, contexts, table, **bounds)
+        assert torch.equal(cache.attend(q, starts, contexts, table, **bounds), whole)
+        for i in (0, 1, 4):
+            q2, c2 = torch.randn_like(q), torch.ones_like(contexts) * 3
+            a, b = int(starts[i]), int(starts[i + 1])
+            q2[a:b], c2[i] = q[a:b], contexts[i]
+            assert torch.equal(cache.attend(q2, starts, c2, table, **bounds)[a:b], whole[a:b])
 
 
 @pytest.mark.parametrize("new", [1, 60])

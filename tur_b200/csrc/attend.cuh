@@ -24,6 +24,7 @@ struct AttendArgs {
   int* status;
   float *part, *part_ml;  // pieces of rows on their way to the kernel that joins them
   int max_chunks, part_rows;
+  int chunk;              // keys of a chunk of a single token's context
 };
 
 __device__ __forceinline__ void report(int* status, int code) { *reinterpret_cast<volatile int*>(status) = code; }

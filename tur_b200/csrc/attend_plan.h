@@ -36,19 +36,25 @@ TQ_HD int64_t keys_seen(const Span& s, int64_t t, bool causal) {
 
 // ---- single tokens: up to TOKEN_ROWS rows (new tokens x query heads of a key head)
 constexpr int TOKEN_ROWS = 16;
-// A context is cut into chunks whose length goes by the context alone: a row's bits do not depend on the
-// other sequences of the call. Up to sixteen chunks of at least 256 keys while that fills a GPU with one
-// sequence of eight heads, not above 1024 keys: a chunk of rows x head_dim f32 leaves the SM and comes back.
-TQ_HD int64_t token_chunk(int64_t ctx) {
-  const int64_t c = (ctx + 1023) / 1024 * 64;  // ctx / 16 in whole 64s
-  return c < 256 ? 256 : c > 1024 ? 1024 : c;
-}
-TQ_HD int64_t token_chunks(int64_t ctx) { return ctx <= 0 ? 1 : (ctx + token_chunk(ctx) - 1) / token_chunk(ctx); }
-// The most chunks that any context up to max_context has (the count falls by one where the length steps up).
-TQ_HD int64_t token_chunks_max(int64_t max_context) {
-  if (max_context <= 4096) return token_chunks(max_context);
-  const int64_t n = (max_context + 1023) / 1024;
-  return n < 16 ? 16 : n;
+// The contexts of a call are cut into chunks of one length, a CTA each, three CTAs at a time on an SM. A CTA has
+// costs of its own (the way from the lengths over the page table to the first keys, the join of its warps) worth
+// TOKEN_OVERHEAD keys, and the last wave is as long as a full one, so the length is the one whose waves x (keys +
+// overhead) is least. Measured, us a call (bf16 24 x 4096, Q8_0 24 x 4096, f16 2 x 120000 keys; 8 heads of 128): 256 keys
+// 81, 92, -; 512 keys 76, 76, 176; 1024 keys 70, 69, 189; the rule's own 70, 69, 173.
+constexpr int TOKEN_STEP = 128, TOKEN_CHUNK_MAX = 8192, TOKEN_OVERHEAD = 96, TOKEN_CTAS = 3;
+inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64_t max_context, int sms) {
+  int64_t best = TOKEN_STEP, cost = -1;
+  for (int64_t c = TOKEN_STEP; c <= TOKEN_CHUNK_MAX; c += TOKEN_STEP) {
+    const int64_t chunks = max_context <= c ? 1 : (max_context + c - 1) / c, slots = (int64_t)TOKEN_CTAS * sms;
+    const int64_t keys = c < max_context ? c : max_context;
+    const int64_t t = (pairs * chunks + slots - 1) / slots * (keys + TOKEN_OVERHEAD);
+    if (cost < 0 || t < cost) {
+      cost = t;
+      best = c;
+    }
+    if (c >= max_context) break;
+  }
+  return best;
 }
 
 }  // namespace turq

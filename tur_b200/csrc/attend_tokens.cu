@@ -1,15 +1,20 @@
 // Attention of single tokens (up to 16 rows = new tokens x query heads of one key head): bound by the bytes of
 // K and V, which every row of a key head shares.
 //
-// A CTA takes one chunk (token_chunk) of one key head of one sequence, its four warps every fourth step of 16 to 64
-// keys. A warp copies its own steps by TMA into its own ring (no CTA-wide barrier in the loop), multiplies with
-// mma.sync (rows x keys: 16 x 8 tiles; the rows are few, so the matrix rate does not matter and the accumulators stay
-// in registers) and keeps its own running maximum, sum and output; the four are joined through shared memory at the
-// end. A context of one chunk is then finished; the pieces of a longer one go to the workspace and
-// join_tokens_kernel adds them in chunk order.
+// A CTA takes one chunk (plan_token_chunk) of one key head of one sequence, its four warps every fourth step of 16 to 64
+// keys. A warp copies its own steps by TMA into its own ring (no CTA-wide barrier in the loop) and keeps its own running
+// maximum, sum and output; the four are joined through shared memory at the end. A context of one chunk is then finished;
+// the pieces of a longer one go to the workspace and join_tokens_kernel adds them in chunk order.
 //
-// Q8_0 keys and values are converted to f16 (2^-11 of a value, against 2^-8 of a block's largest that the
-// quantization itself costs) in registers; weights are rounded to the 16-bit type before they meet V.
+// Products are transposed, S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16: keys and value columns fill the 16 rows of
+// the wide operand, query rows the 8 columns of the narrow one (one or two tiles of it). The rows are few, so the matrix
+// rate does not matter, the accumulators stay in registers, and every key and value is brought into an operand once:
+// 16-bit ones by ldmatrix, Q8_0 ones from int8 in registers. There the order of k (of the head's elements) and of m
+// (of the value's columns) is the one in which a lane's 16 bytes lie: lane (g, c) multiplies bytes D/4 c .. of keys g and
+// g + 8, and columns D/8 g .. of the values of its four keys.
+//
+// Q8_0 keys and values are rounded to f16 (2^-11 of a value, against the 2^-8 of a block's largest that the
+// quantization itself costs); weights are rounded to the 16-bit type before they meet V.
 #include "attend.cuh"
 #include "attend_launch.h"
 #include "tc_common.cuh"
@@ -18,7 +23,7 @@
 namespace turq {
 
 constexpr int TOK_WARPS = 4;
-constexpr int TOK_STAGES = 3;
+constexpr int TOK_STAGES = 2;
 
 // The bytes of a step: 8 KB of keys and values, with the scales of Q8_0 behind them.
 template <int D, bool Q8> struct TokGeom {
@@ -28,10 +33,10 @@ template <int D, bool Q8> struct TokGeom {
   static constexpr int SC = Q8 ? 16 * (D / 32) * 2 : 0;  // scales of 16 keys: 128 or 64 bytes,
   static constexpr int SC_AT = Q8 ? 128 : 0;             // each copy to a 128-byte boundary, as tensor copies ask for
   static constexpr int STAGE = 8192 + (Q8 ? 1024 : 0);
-  static constexpr int SCRATCH = Q8 ? 16 * D * 2 : 0;  // 16 values of V as f16
-  static constexpr int RING = TOK_STAGES * STAGE + SCRATCH;
+  static constexpr int RING = TOK_STAGES * STAGE;
+  static constexpr int RES = D + 4;                    // floats from one result row to the next: four row pairs x eight columns meet all banks
   static_assert(KEYS / 16 * 2 * SC_AT <= 1024 && SC <= 128, "scales of a step");
-  static_assert(RING >= 16 * D * 4 + 128, "the ring holds a warp's result");
+  static_assert(RING >= 16 * RES * 4 + 128, "the ring holds a warp's result");
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -77,50 +82,55 @@ __device__ __forceinline__ void copy_box2(uint32_t dst, const CUtensorMap* map, 
 
 struct TokMaps { CUtensorMap k, v, ks, vs; };
 
-constexpr int TOK_CHUNK_MAX = 1024;
-
-template <int D, bool Q8, bool BF>
-__global__ void __launch_bounds__(32 * TOK_WARPS, 2) attend_tokens_kernel(const __grid_constant__ TokMaps maps, const __grid_constant__ AttendArgs a) {
+template <int D, bool Q8, bool BF, int NR /* tiles of 8 query rows */>
+__global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kernel(const __grid_constant__ TokMaps maps, const __grid_constant__ AttendArgs a) {
   using G = TokGeom<D, Q8>;
-  constexpr int KEYS = G::KEYS, NT = KEYS / 8, KS = D / 16, DT = D / 8, G16 = KEYS / 16, HALVES = Q8 ? 1 : D / 64;
+  constexpr int KEYS = G::KEYS, KT = KEYS / 16, KS = D / 16, MT = D / 16, HALVES = Q8 ? 1 : D / 64;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full[TOK_WARPS][TOK_STAGES];
-  __shared__ int pages[TOK_CHUNK_MAX / 16];
+  __shared__ int pages[TOKEN_CHUNK_MAX / 16];
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int chunk = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
-  const Span sp = span_of(a, seq);
-  const int rows = (int)sp.n * a.group;
-  if (sp.n <= 0 || sp.n * a.group > TOKEN_ROWS) return;  // none, or the other kernel's
-  const int64_t len = token_chunk(sp.ctx), lo = chunk * len;
-  if (lo >= sp.ctx && chunk > 0) return;
-  const int keys = (int)max((int64_t)0, min(len, sp.ctx - lo));  // of this chunk
-  const int steps = (keys + KEYS - 1) / KEYS;
-
-  // pages of the chunk: of 16 keys each; none (-1) where the table names none of the cache's
-  const int shift = a.cache.page_shift;
-  for (int i = threadIdx.x; i < (keys + 15) / 16; i += 32 * TOK_WARPS) {
-    const int64_t page = a.page_table[seq * a.table_stride + ((lo + 16 * i) >> shift)];
-    const bool known = page >= 0 && page < a.cache.n_pages;
-    if (!known) report(a.status, TURQ_E_INVALID_ARG);
-    pages[i] = known ? (int)(page * a.cache.n_heads + head) : (int)(a.cache.n_pages * a.cache.n_heads);
-  }
+  const int64_t lo = (int64_t)chunk * a.chunk;
   const uint32_t base = (s_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = base + warp * G::RING;
-  if (threadIdx.x == 0) abort_flag = 0;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+  }
   if (lane == 0) {
     for (int s = 0; s < TOK_STAGES; s++) bar_init(&full[warp][s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // launched behind its predecessor's last block: everything that kernels before it wrote is read from here on
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // Pages of the chunk, 16 keys each, at the same time as the lengths: entries behind the context are dropped afterwards.
+  const int shift = a.cache.page_shift, most = (int)min((int64_t)a.chunk, a.max_context - lo);
+  for (int i = threadIdx.x; i < (most + 15) / 16; i += 32 * TOK_WARPS) pages[i] = a.page_table[seq * a.table_stride + ((lo + 16 * i) >> shift)];
+  const Span sp = span_of(a, seq);
+  const int rows = (int)sp.n * a.group;
+  if (sp.n <= 0 || sp.n * a.group > TOKEN_ROWS) return;  // none, or the other kernel's
+  if (lo >= sp.ctx && chunk > 0) return;
+  const int keys = (int)max((int64_t)0, min((int64_t)a.chunk, sp.ctx - lo));  // of this chunk
+  const int steps = (keys + KEYS - 1) / KEYS;
   __syncthreads();
 
-  // one step's copies: only boxes that begin inside the context
+  // one step's copies: only boxes that begin inside the context; a page that the cache does not have reads as zeros
   auto issue = [&](int step, int stage) {
-    const int k0 = step * KEYS, boxes = min(G16, (keys - k0 + 15) / 16);
+    const int k0 = step * KEYS, boxes = min(KT, (keys - k0 + 15) / 16);
     const uint32_t bar = s_u32(&full[warp][stage]), at = ring + stage * G::STAGE;
     bar_expect_tx(&full[warp][stage], boxes * (2 * HALVES * G::BOX + 2 * G::SC));
-    for (int b = 0; b < boxes; b++) {
-      const int z = pages[k0 / 16 + b], y = (int)((lo + k0 + 16 * b) & (a.cache.page_size - 1));
+#pragma unroll
+    for (int b = 0; b < KT; b++) {
+      if (b >= boxes) break;
+      const int64_t page = pages[k0 / 16 + b];
+      const bool known = page >= 0 && page < a.cache.n_pages;
+      if (!known) report(a.status, TURQ_E_INVALID_ARG);
+      const int z = (int)((known ? page : a.cache.n_pages) * a.cache.n_heads) + (known ? head : 0);
+      const int y = (int)((lo + k0 + 16 * b) & (a.cache.page_size - 1));
 #pragma unroll
       for (int h = 0; h < HALVES; h++) {
         copy_box3(at + (b * HALVES + h) * G::BOX, &maps.k, 64 * h, y, z, bar);
@@ -128,7 +138,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, 2) attend_tokens_kernel(const 
       }
       if (Q8) {
         copy_box2(at + 8192 + b * G::SC_AT, &maps.ks, y * (D / 32), z, bar);
-        copy_box2(at + 8192 + (G16 + b) * G::SC_AT, &maps.vs, y * (D / 32), z, bar);
+        copy_box2(at + 8192 + (KT + b) * G::SC_AT, &maps.vs, y * (D / 32), z, bar);
       }
     }
   };
@@ -136,54 +146,57 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, 2) attend_tokens_kernel(const 
     for (int s = 0; s < TOK_STAGES; s++)
       if (warp + s * TOK_WARPS < steps) issue(warp + s * TOK_WARPS, s);
 
-  // Q as the 16 x 16 operand. On f16 caches a bf16 row is brought to f16 by a power of two that its largest element
-  // fits (the products undo it); rows that do not exist are zeros. The k order is the one in which a lane finds keys:
-  // in order for 16-bit types, a lane's own D / 4 consecutive elements for int8.
-  uint32_t qf[KS][4];
-  float mul[2], seen_f[2];
-  int seen[2];
+  // Q^T, 16 elements x 8 rows: lane (g, c) holds row g. On f16 caches a bf16 row is brought to f16 by a power of two that its
+  // largest element fits (the products undo it); rows that do not exist are zeros.
+  uint32_t qf[NR][KS][2];
+  float mul[NR][2];  // of the rows whose sums this lane holds: 8 j + 2 c + e
+  int seen[NR][2];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int r = g + 8 * i;
+  for (int j = 0; j < NR; j++) {
+    const int r = 8 * j + g;
     const bool live = r < rows;
-    const int t = live ? r / a.group : 0, h = head * a.group + (live ? r % a.group : 0);
-    const uint16_t* qp = a.q + (sp.first + t) * a.q_stride + (int64_t)h * D;
-    seen[i] = live ? (int)max((int64_t)0, min((int64_t)keys, keys_seen(sp, t, a.causal) - lo)) : 0;
+    const uint16_t* qp = a.q + (sp.first + (live ? r / a.group : 0)) * a.q_stride + (int64_t)(head * a.group + (live ? r % a.group : 0)) * D;
 #pragma unroll
-    for (int s = 0; s < KS; s++) {
+    for (int s = 0; s < KS; s++)
 #pragma unroll
-      for (int p = 0; p < 2; p++) {
-        const int d0 = Q8 ? (D / 4) * c + 4 * s + 2 * p : 16 * s + 2 * c + 8 * p;
-        qf[s][i + 2 * p] = live ? *reinterpret_cast<const uint32_t*>(qp + d0) : 0u;
-      }
-    }
-    mul[i] = a.scale_log2;
+      for (int p = 0; p < 2; p++) qf[j][s][p] = live ? *reinterpret_cast<const uint32_t*>(qp + (Q8 ? (D / 4) * c + 4 * s + 2 * p : 16 * s + 2 * c + 8 * p)) : 0u;
+    float f = a.scale_log2;
     if (!BF && a.q_bf16) {
       uint32_t top = 0;  // exponent and fraction of the largest magnitude
 #pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int p = 0; p < 2; p++) top = max(top, max(qf[s][i + 2 * p] & 0x7FFFu, (qf[s][i + 2 * p] >> 16) & 0x7FFFu));
+        for (int p = 0; p < 2; p++) top = max(top, max(qf[j][s][p] & 0x7FFFu, (qf[j][s][p] >> 16) & 0x7FFFu));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       const int e = min(max((int)(top >> 7) - 127, -100), 100);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      mul[i] *= __uint_as_float((uint32_t)(127 + e) << 23);
+      f *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int p = 0; p < 2; p++) {
-          const uint32_t w = qf[s][i + 2 * p];
-          qf[s][i + 2 * p] = pack16<false>(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down);
+          const uint32_t w = qf[j][s][p];
+          qf[j][s][p] = pack16<false>(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xFFFF0000u) * down);
         }
     }
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int row = 8 * j + 2 * c + e;
+      mul[j][e] = __shfl_sync(0xFFFFFFFFu, f, 4 * (2 * c + e));
+      seen[j][e] = row < rows ? (int)max((int64_t)0, min((int64_t)keys, keys_seen(sp, row / a.group, a.causal) - lo)) : 0;
+    }
   }
-  (void)seen_f;
   const int least = a.causal ? (int)max((int64_t)0, min((int64_t)keys, keys_seen(sp, 0, true) - lo)) : keys;  // keys that every row sees
 
-  float o[DT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[NR][MT][4], m[NR][2], l[NR][2];
 #pragma unroll
-  for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int j = 0; j < NR; j++) {
+#pragma unroll
+    for (int i = 0; i < MT; i++) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+    m[j][0] = m[j][1] = -INFINITY;
+    l[j][0] = l[j][1] = 0.f;
+  }
   bool dead = false;
   const int r8 = lane & 7, mi = lane >> 3;
 
@@ -196,93 +209,107 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, 2) attend_tokens_kernel(const 
     __syncwarp();
     const uint32_t at = ring + stage * G::STAGE;
     const int k0 = step * KEYS;
-    const bool tail = keys - k0 < KEYS;
 
-    float s[NT][4];
+    // S^T: lane (g, c) gets keys g and g + 8 of a tile for rows 2c, 2c + 1
+    float s[KT][NR][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    for (int kt = 0; kt < KT; kt++) {
+#pragma unroll
+      for (int j = 0; j < NR; j++) s[kt][j][0] = s[kt][j][1] = s[kt][j][2] = s[kt][j][3] = 0.f;
       if (!Q8) {
 #pragma unroll
-        for (int q4 = 0; q4 < D / 32; q4++) {  // four column chunks of 8 keys: two k steps
-          uint32_t b[4];
-          const int ch = q4 * 4 + mi, row = (nt & 1) * 8 + r8;
-          ldsm4(b, at + ((nt >> 1) * HALVES + (ch >> 3)) * G::BOX + row * 128 + (((ch & 7) ^ r8) << 4));
-          mma_16816<BF>(s[nt], qf[2 * q4], b[0], b[1]);
-          mma_16816<BF>(s[nt], qf[2 * q4 + 1], b[2], b[3]);
+        for (int i = 0; i < KS; i++) {
+          uint32_t k[4];
+          const int ch = 2 * i + (mi >> 1), row = (mi & 1) * 8 + r8;
+          ldsm4(k, at + (kt * HALVES + (ch >> 3)) * G::BOX + row * 128 + (((ch & 7) ^ r8) << 4));
+#pragma unroll
+          for (int j = 0; j < NR; j++) mma_16816<BF>(s[kt][j], k, qf[j][i][0], qf[j][i][1]);
         }
       } else {
-        // lane (g, c): key g, elements (D / 4) c ..: one block of 32 (D = 128) or half of one
-        const int row = (nt & 1) * 8 + g;
-        const uint32_t kb = at + (nt >> 1) * G::BOX + row * D;
-        uint16_t sc;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc) : "r"(at + 8192 + (nt >> 1) * G::SC_AT + (row * (D / 32) + c * D / 128) * 2));
-        const __half2 scale = __half2half2(__ushort_as_half(sc));
+        const uint32_t kb = at + kt * G::BOX + g * D, sb = at + 8192 + kt * G::SC_AT + (g * (D / 32) + c * D / 128) * 2;
+        uint16_t s0, s1;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s0) : "r"(sb));
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s1) : "r"(sb + 8 * (D / 32) * 2));
+        const __half2 sc0 = __half2half2(__ushort_as_half(s0)), sc1 = __half2half2(__ushort_as_half(s1));
 #pragma unroll
-        for (int q4 = 0; q4 < D / 64; q4++) {  // 16 bytes: four k steps
-          const int ch = c * (D / 64) + q4;
-          uint4 w;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                       : "r"(kb + ((D == 128 ? (ch ^ (row & 7)) : ch) << 4)));
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        for (int q4 = 0; q4 < D / 64; q4++) {  // 16 bytes of each of the two keys: four k steps
+          const int ch = c * (D / 64) + q4, at16 = (D == 128 ? ch ^ g : ch ^ ((g >> 1) & 3)) << 4;
+          uint32_t w0[4], w1[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w0[0]), "=r"(w0[1]), "=r"(w0[2]), "=r"(w0[3]) : "r"(kb + at16));
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w1[0]), "=r"(w1[1]), "=r"(w1[2]), "=r"(w1[3]) : "r"(kb + 8 * D + at16));
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            uint32_t b0, b1;
-            halves_of(ww[i], scale, b0, b1);
-            mma_16816<BF>(s[nt], qf[4 * q4 + i], b0, b1);
+            uint32_t k[4];
+            halves_of(w0[i], sc0, k[0], k[2]);
+            halves_of(w1[i], sc1, k[1], k[3]);
+#pragma unroll
+            for (int j = 0; j < NR; j++) mma_16816<BF>(s[kt][j], k, qf[j][4 * q4 + i][0], qf[j][4 * q4 + i][1]);
           }
         }
       }
     }
     // weights
-    float top[2] = {m[0], m[1]};
-    const bool mask = k0 + KEYS > least;
+    float top[NR][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
+    for (int j = 0; j < NR; j++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float x = s[nt][e] * mul[e >> 1];
-        if (mask && k0 + 8 * nt + 2 * c + (e & 1) >= seen[e >> 1]) x = -INFINITY;
-        s[nt][e] = x;
-        top[e >> 1] = fmaxf(top[e >> 1], x);
+      for (int e = 0; e < 2; e++) {
+        top[j][e] = m[j][e];
+#pragma unroll
+        for (int kt = 0; kt < KT; kt++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float& x = s[kt][j][2 * h + e];
+            x *= mul[j][e];
+            if (k0 + KEYS > least && k0 + 16 * kt + 8 * h + g >= seen[j][e]) x = -INFINITY;
+            top[j][e] = fmaxf(top[j][e], x);
+          }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top[j][e] = fmaxf(top[j][e], __shfl_xor_sync(0xFFFFFFFFu, top[j][e], d));
       }
-    float was[2];
+    bool grew = false;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 2));
+    for (int j = 0; j < NR; j++) grew = grew || top[j][0] > m[j][0] || top[j][1] > m[j][1];
+    if (__any_sync(0xFFFFFFFFu, grew)) {
+#pragma unroll
+      for (int j = 0; j < NR; j++) {
+        float was[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          was[e] = m[j][e] == -INFINITY ? 0.f : ex2(m[j][e] - top[j][e]);
+          m[j][e] = top[j][e];
+          l[j][e] *= was[e];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          o[j][i][0] *= was[0]; o[j][i][1] *= was[1];
+          o[j][i][2] *= was[0]; o[j][i][3] *= was[1];
+        }
+      }
     }
-    if (__any_sync(0xFFFFFFFFu, top[0] > m[0] || top[1] > m[1])) {
+    // P^T: the two 8 x 8 tiles of 16 keys turned round
+    uint32_t p[KT][NR][2];
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        was[i] = m[i] == -INFINITY ? 0.f : ex2(m[i] - top[i]);
-        m[i] = top[i];
-        l[i] *= was[i];
-      }
+    for (int j = 0; j < NR; j++) {
+      const float sub[2] = {m[j][0] == -INFINITY ? 0.f : m[j][0], m[j][1] == -INFINITY ? 0.f : m[j][1]};
 #pragma unroll
-      for (int i = 0; i < DT; i++) {
-        o[i][0] *= was[0]; o[i][1] *= was[0];
-        o[i][2] *= was[1]; o[i][3] *= was[1];
+      for (int kt = 0; kt < KT; kt++) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float x = ex2(s[kt][j][2 * h] - sub[0]), y = ex2(s[kt][j][2 * h + 1] - sub[1]);
+          l[j][0] += x;
+          l[j][1] += y;
+          asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[kt][j][h]) : "r"(pack16<BF>(x, y)));
+        }
       }
     }
-    const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        s[nt][e] = ex2(s[nt][e] - sub[e >> 1]);
-        l[e >> 1] += s[nt][e];
-      }
     // values, 16 keys at a time
 #pragma unroll
-    for (int b = 0; b < G16; b++) {
-      const uint32_t p[4] = {pack16<BF>(s[2 * b][0], s[2 * b][1]), pack16<BF>(s[2 * b][2], s[2 * b][3]), pack16<BF>(s[2 * b + 1][0], s[2 * b + 1][1]),
-                             pack16<BF>(s[2 * b + 1][2], s[2 * b + 1][3])};
-      const int live = keys - k0 - 16 * b;  // keys of this box that exist: what lies behind may be anything, and 0 x NaN is NaN
-      uint32_t vb;
+    for (int kt = 0; kt < KT; kt++) {
+      const int live = keys - k0 - 16 * kt;  // keys of this box that exist: what lies behind may be anything, and 0 x NaN is NaN
       if (!Q8) {
-        vb = at + 4096 + b * HALVES * G::BOX;
-        if (tail && live < 16) {
+        const uint32_t vb = at + 4096 + kt * HALVES * G::BOX;
+        if (live < 16) {
           for (int i = lane; i < 16 * D / 8; i += 32) {
             const int row = i & 15, ch = i >> 4;
             if (row >= live)
@@ -290,89 +317,94 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, 2) attend_tokens_kernel(const 
           }
           __syncwarp();
         }
-      } else {
-        vb = ring + TOK_STAGES * G::STAGE;
-        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) {  // 16 bytes of a value: 16 x D / 16 of them
-          const int id = i * 32 + lane, row = id / (D / 16), ch = id % (D / 16);
-          uint4 w;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                       : "r"(at + 4096 + b * G::BOX + row * D + ((D == 128 ? (ch ^ (row & 7)) : ch) << 4)));
-          uint16_t sc;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc) : "r"(at + 8192 + (G16 + b) * G::SC_AT + (row * (D / 32) + (ch >> 1)) * 2));
-          __half2 scale = __half2half2(__ushort_as_half(sc));
-          uint32_t h[8];
-          halves_of(w.x, scale, h[0], h[1]);
-          halves_of(w.y, scale, h[2], h[3]);
-          halves_of(w.z, scale, h[4], h[5]);
-          halves_of(w.w, scale, h[6], h[7]);
-          if (row >= live) {
+        for (int i = 0; i < MT; i++) {
+          uint32_t v[4];
+          const int row = (mi >> 1) * 8 + r8, ch = 2 * i + (mi & 1);
+          ldsm4t(v, vb + (ch >> 3) * G::BOX + row * 128 + (((ch & 7) ^ r8) << 4));
 #pragma unroll
-            for (int e = 0; e < 8; e++) h[e] = 0u;
-          }
-          // 64-column blocks of 16 rows, 16-byte chunks in the order of the 128-byte swizzle
-          const uint32_t dst = vb + (ch >> 2) * 2048 + row * 128;
-          const int c0 = (2 * ch) & 7;
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + ((c0 ^ (row & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (((c0 + 1) ^ (row & 7)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+          for (int j = 0; j < NR; j++) mma_16816<BF>(o[j][i], v, p[kt][j][0], p[kt][j][1]);
         }
-        __syncwarp();
-      }
+      } else {
+        // Lane (g, c): D / 8 columns from D/8 g of keys 2c, 2c + 1, 2c + 8, 2c + 9; tile i's rows g and g + 8 are its columns 2i and
+        // 2i + 1. Behind the context's end the quants are some bytes, and a scale of zero makes them zeros.
+        const uint32_t vb = at + 4096 + kt * G::BOX, sb = at + 8192 + (KT + kt) * G::SC_AT + (g * D / 256) * 2;
+        constexpr int W = D / 32;  // words of a key
+        uint32_t w[4][W];
+        uint16_t sc[4];
 #pragma unroll
-      for (int dt = 0; dt < DT; dt += 2) {
-        uint32_t v[4];
-        const int row = (mi & 1) * 8 + r8, ch = dt + (mi >> 1);
-        ldsm4t(v, vb + (ch >> 3) * 2048 + row * 128 + (((ch & 7) ^ r8) << 4));
-        mma_16816<BF>(o[dt], p, v[0], v[1]);
-        mma_16816<BF>(o[dt + 1], p, v[2], v[3]);
+        for (int i = 0; i < 4; i++) {
+          const int row = 2 * c + (i & 1) + 8 * (i >> 1);
+          if (D == 128)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2 % W]), "=r"(w[i][3 % W])
+                         : "r"(vb + row * D + ((g ^ (row & 7)) << 4)));
+          else
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[i][0]), "=r"(w[i][1])
+                         : "r"(vb + row * D + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8));
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[i]) : "r"(sb + row * (D / 32) * 2));
+          if (row >= live) sc[i] = 0;
+        }
+        const __half2 sc01 = __halves2half2(__ushort_as_half(sc[0]), __ushort_as_half(sc[1])), sc23 = __halves2half2(__ushort_as_half(sc[2]), __ushort_as_half(sc[3]));
+        const __half2 off = __float2half2_rn(1152.f);
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+          const uint32_t x0 = w[0][i] ^ 0x80808080u, x1 = w[1][i] ^ 0x80808080u, x2 = w[2][i] ^ 0x80808080u, x3 = w[3][i] ^ 0x80808080u;
+#pragma unroll
+          for (int h = 0; h < 2; h++) {  // columns 4i + 2h, + 1
+            const uint32_t a01 = __byte_perm(x0, x1, h ? 0x7362 : 0x5140), a23 = __byte_perm(x2, x3, h ? 0x7362 : 0x5140);
+            uint32_t v[4];
+            v[0] = h22u(__hmul2(__hsub2(pair01(a01), off), sc01));
+            v[1] = h22u(__hmul2(__hsub2(pair23(a01), off), sc01));
+            v[2] = h22u(__hmul2(__hsub2(pair01(a23), off), sc23));
+            v[3] = h22u(__hmul2(__hsub2(pair23(a23), off), sc23));
+#pragma unroll
+            for (int j = 0; j < NR; j++) mma_16816<BF>(o[j][2 * i + h], v, p[kt][j][0], p[kt][j][1]);
+          }
+        }
       }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // this stage was read, at a context's end also written, by ordinary accesses
     __syncwarp();
-    if (lane == 0 && step + TOK_STAGES * TOK_WARPS < steps) {
-      // this stage was read (and, at a tail that no later step follows, written) by ordinary accesses
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      issue(step + TOK_STAGES * TOK_WARPS, stage);
-    }
+    if (lane == 0 && step + TOK_STAGES * TOK_WARPS < steps) issue(step + TOK_STAGES * TOK_WARPS, stage);
   }
 
   // the four warps' results: each into its own ring, whose copies have all arrived
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], 2);
-  }
   __syncwarp();
-  uint8_t* const mine = raw + (ring - s_u32(raw));
-  float* const ro = reinterpret_cast<float*>(mine);
-  float* const rml = ro + 16 * D;
+  float* const ro = reinterpret_cast<float*>(raw + (ring - s_u32(raw)));
+  float* const rml = ro + 16 * G::RES;
 #pragma unroll
-  for (int dt = 0; dt < DT; dt++) {
-    *reinterpret_cast<float2*>(ro + g * D + 8 * dt + 2 * c) = make_float2(o[dt][0], o[dt][1]);
-    *reinterpret_cast<float2*>(ro + (g + 8) * D + 8 * dt + 2 * c) = make_float2(o[dt][2], o[dt][3]);
-  }
-  if (c == 0) {
+  for (int j = 0; j < NR; j++) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      rml[2 * (g + 8 * i)] = m[i];
-      rml[2 * (g + 8 * i) + 1] = l[i];
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[j][e] += __shfl_xor_sync(0xFFFFFFFFu, l[j][e], d);
+      const int row = 8 * j + 2 * c + e;
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        ro[row * G::RES + (Q8 ? D / 8 * g + 2 * i : 16 * i + g)] = o[j][i][e];
+        ro[row * G::RES + (Q8 ? D / 8 * g + 2 * i + 1 : 16 * i + g + 8)] = o[j][i][2 + e];
+      }
+      if (g == 0) {
+        rml[2 * row] = m[j][e];
+        rml[2 * row + 1] = l[j][e];
+      }
     }
   }
   __syncthreads();
-  const bool whole = len >= sp.ctx;
+  const bool whole = sp.ctx <= a.chunk;
   const int64_t item = ((int64_t)seq * a.cache.n_heads + head) * a.max_chunks + chunk;
   const float* const rb = reinterpret_cast<const float*>(raw + (base - s_u32(raw)));
   for (int i = threadIdx.x; i < rows * (D / 2); i += 32 * TOK_WARPS) {
     const int r = i / (D / 2), d = 2 * (i % (D / 2));
     float mm = -INFINITY, ll = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int w = 0; w < TOK_WARPS; w++) mm = fmaxf(mm, rb[w * (G::RING / 4) + 16 * D + 2 * r]);
+    for (int w = 0; w < TOK_WARPS; w++) mm = fmaxf(mm, rb[w * (G::RING / 4) + 16 * G::RES + 2 * r]);
 #pragma unroll
     for (int w = 0; w < TOK_WARPS; w++) {
       const float* p = rb + w * (G::RING / 4);
-      const float f = mm == -INFINITY ? 0.f : ex2(p[16 * D + 2 * r] - mm);
-      const float2 v = *reinterpret_cast<const float2*>(p + r * D + d);
-      ll += f * p[16 * D + 2 * r + 1];
+      const float f = mm == -INFINITY ? 0.f : ex2(p[16 * G::RES + 2 * r] - mm);
+      const float2 v = *reinterpret_cast<const float2*>(p + r * G::RES + d);
+      ll += f * p[16 * G::RES + 2 * r + 1];
       x += f * v.x;
       y += f * v.y;
     }
@@ -387,38 +419,62 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, 2) attend_tokens_kernel(const 
   }
 }
 
-// The pieces of one key head of a sequence, in chunk order. D / 2 threads a row.
+// The pieces of a row, in chunk order: a CTA per row, whose warps take every eighth piece and are added in their order. Its lanes
+// first read all maxima and sums at once (a loop over pieces would be as many trips to memory, one behind the other).
 template <int D>
 __global__ void __launch_bounds__(256) join_tokens_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int WARPS = 8, E = D / 32;
+  __shared__ float sh[WARPS][D], sh_l[WARPS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int head = blockIdx.x, seq = blockIdx.y;
+  const int r = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Span sp = cut_span(a.starts[seq], a.starts[seq + 1], a.contexts[seq], a.n_tokens, a.max_new, a.max_context);
-  const int64_t len = token_chunk(sp.ctx);
-  if (sp.n <= 0 || sp.n * a.group > TOKEN_ROWS || len >= sp.ctx) return;
-  const int rows = (int)sp.n * a.group, chunks = (int)token_chunks(sp.ctx);
+  if (sp.n <= 0 || sp.n * a.group > TOKEN_ROWS || sp.ctx <= a.chunk || r >= sp.n * a.group) return;
+  const int chunks = (int)((sp.ctx + a.chunk - 1) / a.chunk);
   const int64_t item0 = ((int64_t)seq * a.cache.n_heads + head) * a.max_chunks;
-  for (int i = threadIdx.x; i < rows * (D / 2); i += 256) {
-    const int r = i / (D / 2), d = 2 * (i % (D / 2));
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + item0 * a.part_rows + r;
-    const float* po = a.part + (item0 * a.part_rows + r) * D + d;
-    float mm = -INFINITY, ll = 0.f, x = 0.f, y = 0.f;
-    for (int k = 0; k < chunks; k++) mm = fmaxf(mm, ml[(int64_t)k * a.part_rows].x);
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + item0 * a.part_rows + r;
+  const float* po = a.part + (item0 * a.part_rows + r) * D + lane * E;
+  float mm = -INFINITY;
+  for (int k = lane; k < chunks; k += 32) mm = fmaxf(mm, ml[(int64_t)k * a.part_rows].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, d));
+  const float sub = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = 0.f;
 #pragma unroll 4
-    for (int k = 0; k < chunks; k++) {
-      const float2 t = ml[(int64_t)k * a.part_rows], v = *reinterpret_cast<const float2*>(po + (int64_t)k * a.part_rows * D);
-      const float f = mm == -INFINITY ? 0.f : ex2(t.x - mm);
-      ll += f * t.y;
-      x += f * v.x;
-      y += f * v.y;
+  for (int k = warp; k < chunks; k += WARPS) {
+    const float2 t = ml[(int64_t)k * a.part_rows];
+    const float f = ex2(t.x - sub);
+    ll += f * t.y;
+    const float* p = po + (int64_t)k * a.part_rows * D;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p + e);
+      o[e] += f * v.x;
+      o[e + 1] += f * v.y;
     }
-    const float inv = ll > 0.f ? 1.f / ll : ll == 0.f ? 0.f : ll;
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) sh[warp][lane * E + e] = o[e];
+  if (lane == 0) sh_l[warp] = ll;
+  __syncthreads();
+  const int d = 2 * threadIdx.x;
+  if (d < D) {
+    float x = 0.f, y = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      x += sh[w][d];
+      y += sh[w][d + 1];
+      l += sh_l[w];
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     const int t = r / a.group, h = head * a.group + r % a.group;
     store_out2(a.out, a.out_dtype, ((sp.first + t) * a.hq + h) * D + d, x * inv, y * inv);
   }
 }
 
-template <int D, bool Q8, bool BF>
-static cudaError_t launch_tokens(const turq_kv_cache* kc, const AttendArgs& a, cudaStream_t s, int* launches) {
+template <int D, bool Q8, bool BF, int NR>
+static cudaError_t launch_tokens_rows(const turq_kv_cache* kc, const AttendArgs& a, cudaStream_t s, int* launches) {
   using G = TokGeom<D, Q8>;
   constexpr int SMEM = TOK_WARPS * G::RING + 1024;
   static PerDeviceOnce configured;
@@ -426,17 +482,21 @@ static cudaError_t launch_tokens(const turq_kv_cache* kc, const AttendArgs& a, c
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (!configured.done(dev)) {
-    e = cudaFuncSetAttribute(attend_tokens_kernel<D, Q8, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    e = cudaFuncSetAttribute(attend_tokens_kernel<D, Q8, BF, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     configured.set(dev);
   }
   const TokMaps maps{kc->k16, kc->v16, kc->ks16, kc->vs16};
-  attend_tokens_kernel<D, Q8, BF><<<dim3((unsigned)a.max_chunks, (unsigned)a.cache.n_heads, (unsigned)a.n_seqs), 32 * TOK_WARPS, SMEM, s>>>(maps, a);
-  e = cudaGetLastError();
   (*launches)++;
+  e = launch_pdl(attend_tokens_kernel<D, Q8, BF, NR>, dim3((unsigned)a.max_chunks, (unsigned)a.cache.n_heads, (unsigned)a.n_seqs), dim3(32 * TOK_WARPS), SMEM, s,
+                 maps, a);
   if (e != cudaSuccess || a.max_chunks == 1) return e;
   (*launches)++;
-  return launch_pdl(join_tokens_kernel<D>, dim3((unsigned)a.cache.n_heads, (unsigned)a.n_seqs), dim3(256), 0, s, a);
+  return launch_pdl(join_tokens_kernel<D>, dim3((unsigned)a.part_rows, (unsigned)a.cache.n_heads, (unsigned)a.n_seqs), dim3(256), 0, s, a);
+}
+template <int D, bool Q8, bool BF>
+static cudaError_t launch_tokens(const turq_kv_cache* kc, const AttendArgs& a, cudaStream_t s, int* launches) {
+  return a.part_rows <= 8 ? launch_tokens_rows<D, Q8, BF, 1>(kc, a, s, launches) : launch_tokens_rows<D, Q8, BF, 2>(kc, a, s, launches);
 }
 
 cudaError_t launch_attend_tokens(const turq_kv_cache* kc, const AttendArgs& a, cudaStream_t s, int* launches) {

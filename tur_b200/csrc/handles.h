@@ -56,7 +56,7 @@ struct turq_kv_cache {
   int device = 0;
   int dtype = 0;
   int64_t n_pages = 0;
-  int page_size = 0, n_kv_heads = 0, head_dim = 0;
+  int page_size = 0, n_kv_heads = 0, head_dim = 0, sm_count = 0;
   uint8_t* mem = nullptr;
   bool owns = false;
   size_t off_v = 0, off_ks = 0, off_vs = 0, bytes = 0;

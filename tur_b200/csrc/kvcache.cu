@@ -323,9 +323,8 @@ bool map_planes(turq_kv_cache* kc) {
            map_plane(enc, &kc->k_tile, kc, t, 2, 0, d, 64, whole, CU_TENSOR_MAP_SWIZZLE_128B) &&
            map_plane(enc, &kc->v_tile, kc, t, 2, kc->off_v, d, 64, whole, CU_TENSOR_MAP_SWIZZLE_128B);
   }
-  // Rows of 64 bytes are read without conflicts as they lie. Scales: the 16 tokens' lie one behind the other, so a page
-  // is one row of its head's plane.
-  const CUtensorMapSwizzle swizzle = d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE;
+  // Scales: the 16 tokens' lie one behind the other, so a page is one row of its head's plane.
+  const CUtensorMapSwizzle swizzle = d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   const int per = d / 32;
   auto scales = [&](CUtensorMap* map, size_t offset) {
     const cuuint64_t dims[2] = {(cuuint64_t)kc->page_size * per, (cuuint64_t)kc->n_pages * kc->n_kv_heads};
@@ -430,6 +429,7 @@ int32_t turq_kv_cache_create(turq_ctx* ctx, int32_t dtype, int64_t n_pages, int3
   turq_kv_cache* kc = new (std::nothrow) turq_kv_cache();
   if (!kc) return api_fail(ctx, TURQ_E_INVALID_ARG, "out of host memory");
   kc->device = ctx->device;
+  kc->sm_count = ctx->sm_count;
   kc->dtype = dtype;
   kc->n_pages = n_pages;
   kc->page_size = page_size;
