@@ -25,13 +25,23 @@ _ROW_CODE = {t: int(c) for t, c in _TORCH_TO_GGML.items()}
 
 def _rows(x: torch.Tensor, what: str, device: int, head_dim: int) -> tuple[int, int, int]:
     """(tokens, heads, elements from one token to the next) of a packed operand; refuses what the kernels cannot read."""
+    # A token's calls take a few microseconds on the GPU: what is in order passes with as few questions as possible.
+    if x.dim() == 3 and x.get_device() == device and x.dtype in _ROW_CODE:
+        n, heads, d = x.shape
+        s0, s1, s2 = x.stride()
+        if d == head_dim and s2 == 1 and (s1 == d or heads == 1):
+            return n, heads, s0 if n > 1 else heads * d
+    return _rows_checked(x, what, device, head_dim)
+
+
+def _rows_checked(x: torch.Tensor, what: str, device: int, head_dim: int) -> tuple[int, int, int]:
     if not x.is_cuda or x.get_device() != device:
         raise TurqError(1, f"{what} lives on {x.device}, expected cuda:{device}")
     if x.dtype not in _ROW_CODE:
         raise TurqError(3, f"{what} has dtype {x.dtype}, expected float32, float16 or bfloat16")
     if x.dim() == 3:
         n, heads, d = x.shape
-        dense = (d == 1 or x.stride(2) == 1) and (heads == 1 or x.stride(1) == d)
+        dense = x.stride(2) == 1 and (heads == 1 or x.stride(1) == d)
     elif x.dim() == 2:
         n, d = x.shape[0], head_dim
         heads = x.shape[1] // head_dim
@@ -48,15 +58,17 @@ def _rows(x: torch.Tensor, what: str, device: int, head_dim: int) -> tuple[int, 
 
 
 def _vector(x: torch.Tensor, what: str, device: int, dtype: torch.dtype, n: Optional[int]) -> int:
+    if x.dtype is dtype and x.get_device() == device and x.is_contiguous() and (n is None or x.numel() == n):
+        return x.data_ptr()
     _check_operand(x, what, device, (dtype,))
-    if n is not None and x.numel() != n:
-        raise TurqError(2, f"{what} has {x.numel()} elements, expected {n}")
-    return x.data_ptr()
+    raise TurqError(2, f"{what} has {x.numel()} elements, expected {n}")
 
 
-def _out(x: Optional[torch.Tensor], what: str, shape: tuple, dtype: torch.dtype, device: int) -> torch.Tensor:
+def _out(x: Optional[torch.Tensor], what: str, shape: tuple, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
+    """The output given, or a new one on the device of `like`."""
     if x is None:
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", device))
+        return like.new_empty(shape, dtype=dtype)
+    device = like.get_device()
     _check_operand(x, what, device, (dtype,))
     if x.numel() != math.prod(shape):
         raise TurqError(2, f"{what} has {x.numel()} elements, expected {shape}")
@@ -69,6 +81,8 @@ class RotaryTable:
 
     def __init__(self, table: torch.Tensor, rotary_dim: int, interleaved: bool, ctx: _Context):
         self.table, self.rotary_dim, self.interleaved, self._ctx = table, rotary_dim, interleaved, ctx
+        self._device = table.get_device()
+        self._args = (table.data_ptr(), table.shape[0], rotary_dim, int(interleaved))
 
     @property
     def n_positions(self) -> int:
@@ -122,15 +136,11 @@ class RotaryTable:
         return cls(table, 2 * n, bool(interleaved), ctx)
 
 
-def _rotation(q: torch.Tensor, table: RotaryTable, positions: torch.Tensor, n: int, head_dim: int, dev: int,
-              q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float) -> tuple:
-    """The arguments from the weights to the positions, in the entries' order."""
-    if table.table.get_device() != dev:
+def _weights(table: RotaryTable, head_dim: int, dev: int, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor]) -> tuple:
+    if table._device != dev:
         raise TurqError(1, f"the rotary table lives on {table.table.device}, q on cuda:{dev}")
-    return (_vector(q_weight, "q_weight", dev, torch.float32, head_dim) if q_weight is not None else None,
-            _vector(k_weight, "k_weight", dev, torch.float32, head_dim) if k_weight is not None else None,
-            float(eps), table.table.data_ptr(), table.n_positions, table.rotary_dim, int(table.interleaved),
-            _vector(positions, "positions", dev, torch.int32, n))
+    return (None if q_weight is None else _vector(q_weight, "q_weight", dev, torch.float32, head_dim),
+            None if k_weight is None else _vector(k_weight, "k_weight", dev, torch.float32, head_dim))
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: RotaryTable, *, q_weight: Optional[torch.Tensor] = None,
@@ -149,10 +159,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     out_dtype = out_dtype or q.dtype
     if out_dtype not in _ROW_CODE:
         raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
-    qo, ko = _out(q_out, "q_out", (n, hq, d), out_dtype, dev), _out(k_out, "k_out", (n, hkv, d), out_dtype, dev)
-    st = _lib.load().turq_qk_norm_rope(ctx.handle, q.data_ptr(), qs, k.data_ptr(), ks, _ROW_CODE[q.dtype], n, hq, hkv, d,
-                                       *_rotation(q, table, positions, n, d, dev, q_weight, k_weight, eps), _ROW_CODE[out_dtype],
-                                       qo.data_ptr(), ko.data_ptr(), _stream_ptr(dev))
+    qo, ko = _out(q_out, "q_out", (n, hq, d), out_dtype, q), _out(k_out, "k_out", (n, hkv, d), out_dtype, q)
+    wq, wk = _weights(table, d, dev, q_weight, k_weight)
+    st = _lib.load().turq_qk_norm_rope(ctx.handle, q.data_ptr(), qs, k.data_ptr(), ks, _ROW_CODE[q.dtype], n, hq, hkv, d, wq, wk, eps, *table._args,
+                                       _vector(positions, "positions", dev, torch.int32, n), _ROW_CODE[out_dtype], qo.data_ptr(), ko.data_ptr(),
+                                       _stream_ptr(dev))
     if st != 0:
         ctx.check(st)
     return qo, ko
@@ -164,8 +175,11 @@ class KvCache:
     [n_pages, n_kv_heads, page_size, head_dim] (int8 for Q8_0, with `k_scales`, `v_scales` [..., head_dim / 32]) are views of it."""
 
     def __init__(self, handle: ctypes.c_void_p, memory: torch.Tensor, dtype: GgmlDType, shape: tuple, ctx: _Context):
-        self._h, self.memory, self.dtype, self._ctx = handle, memory, dtype, ctx
+        self._h, self.memory, self.dtype, self._ctx, self._device = handle, memory, dtype, ctx, ctx.device
+        lib = _lib.load()
+        self._append, self._attention, self._workspace = lib.turq_kv_append, lib.turq_kv_attention, lib.turq_kv_attention_workspace
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = shape
+        self._scale = 1.0 / math.sqrt(self.head_dim)
         off = (ctypes.c_int64 * 4)()
         ctx.check(_lib.load().turq_kv_cache_layout(handle, None, off))
         elem = {GgmlDType.F16: torch.float16, GgmlDType.BF16: torch.bfloat16, GgmlDType.Q8_0: torch.int8}[dtype]
@@ -203,7 +217,7 @@ class KvCache:
         return torch.device("cuda", self._ctx.device)
 
     def _kv(self, k: torch.Tensor, v: torch.Tensor) -> tuple:
-        dev, d = self._ctx.device, self.head_dim
+        dev, d = self._device, self.head_dim
         n, hk, ks = _rows(k, "k", dev, d)
         nv, hv, vs = _rows(v, "v", dev, d)
         if hk != self.n_kv_heads or hv != self.n_kv_heads or nv != n or v.dtype != k.dtype:
@@ -215,20 +229,20 @@ class KvCache:
                out_dtype: torch.dtype = torch.bfloat16, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """What attn_q|k|v gave for n new tokens: norms (where a weight is given) and rotation of q and k, k and v into their
         slots (int64 [n]; a negative one is skipped: padding), all in one pass. Returns q [n, heads, d] of out_dtype."""
-        ctx, d = self._ctx, self.head_dim
-        dev = ctx.device
+        dev, d = self._device, self.head_dim
         n, ks, vs = self._kv(k, v)
         nq, hq, qs = _rows(q, "q", dev, d)
         if nq != n or q.dtype != k.dtype:
             raise TurqError(2, f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in tokens and type")
         if out_dtype not in _ROW_CODE:
             raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
-        qo = _out(q_out, "q_out", (n, hq, d), out_dtype, dev)
-        st = _lib.load().turq_kv_append(ctx.handle, self._h, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[q.dtype], n, hq,
-                                        *_rotation(q, table, positions, n, d, dev, q_weight, k_weight, eps),
-                                        _vector(slots, "slots", dev, torch.int64, n), _ROW_CODE[out_dtype], qo.data_ptr(), _stream_ptr(dev))
+        wq, wk = _weights(table, d, dev, q_weight, k_weight)
+        p_positions, p_slots = _vector(positions, "positions", dev, torch.int32, n), _vector(slots, "slots", dev, torch.int64, n)
+        qo = _out(q_out, "q_out", (n, hq, d), out_dtype, q)
+        st = self._append(self._ctx.handle, self._h, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[q.dtype], n, hq, wq, wk, eps,
+                          *table._args, p_positions, p_slots, _ROW_CODE[out_dtype], qo.data_ptr(), _stream_ptr(dev))
         if st != 0:
-            ctx.check(st)
+            self._ctx.check(st)
         return qo
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -243,7 +257,7 @@ class KvCache:
         dev, n = self._ctx.device, slots.numel()
         if out_dtype not in _ROW_CODE:
             raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
-        k, v = (_out(None, "", (n, self.n_kv_heads, self.head_dim), out_dtype, dev) for _ in range(2))
+        k, v = (_out(None, "", (n, self.n_kv_heads, self.head_dim), out_dtype, self.memory) for _ in range(2))
         self._ctx.check(_lib.load().turq_kv_read(self._ctx.handle, self._h, _vector(slots, "slots", dev, torch.int64, None), n,
                                                  _ROW_CODE[out_dtype], k.data_ptr(), v.data_ptr(), _stream_ptr(dev)))
         return k, v
@@ -256,10 +270,9 @@ class KvCache:
         ones last) lies in the pages page_table[i] (int32 [n_seqs, pages]). scale: 1 / sqrt(d) by default. Single tokens,
         chunks and whole prompts go together; max_new and max_context are the longest of each that the call may meet (the
         values on the device are not read here). `out` keeps its rows that belong to no sequence."""
-        ctx, d = self._ctx, self.head_dim
-        dev = ctx.device
+        dev, d = self._device, self.head_dim
         n, hq, qs = _rows(q, "q", dev, d)
-        _check_operand(page_table, "page_table", dev, (torch.int32,))
+        p_table = _vector(page_table, "page_table", dev, torch.int32, None)
         if page_table.dim() != 2:
             raise TurqError(2, f"page_table must be [n_seqs, pages], got {tuple(page_table.shape)}")
         n_seqs, pages = page_table.shape
@@ -270,15 +283,14 @@ class KvCache:
         out_dtype = (out.dtype if out is not None else q.dtype) if out_dtype is None else out_dtype
         if out_dtype not in _ROW_CODE:
             raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
-        y = _out(out, "out", (n, hq, d), out_dtype, dev)
-        lib = _lib.load()
-        nbytes = lib.turq_kv_attention_workspace(self._h, n, n_seqs, hq, max_new, max_context)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=y.device).data_ptr() if nbytes else None
-        st = lib.turq_kv_attention(ctx.handle, self._h, q.data_ptr(), qs, _ROW_CODE[q.dtype], n, hq, p_starts, p_contexts, page_table.data_ptr(),
-                                   pages, n_seqs, max_new, max_context, 1.0 / math.sqrt(d) if scale is None else float(scale), int(causal),
-                                   _ROW_CODE[out_dtype], y.data_ptr(), ws, nbytes, _stream_ptr(dev))
+        y = _out(out, "out", (n, hq, d), out_dtype, q)
+        nbytes = self._workspace(self._h, n, n_seqs, hq, max_new, max_context)
+        ws = y.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        st = self._attention(self._ctx.handle, self._h, q.data_ptr(), qs, _ROW_CODE[q.dtype], n, hq, p_starts, p_contexts, p_table, pages, n_seqs,
+                             max_new, max_context, self._scale if scale is None else scale, causal, _ROW_CODE[out_dtype], y.data_ptr(),
+                             ws.data_ptr() if nbytes else None, nbytes, _stream_ptr(dev))
         if st != 0:
-            ctx.check(st)
+            self._ctx.check(st)
         return y if y.dim() == 3 else y.view(n, hq, d)
 
 

@@ -15,16 +15,19 @@ namespace turq {
 struct AttendWorkspace {
   size_t off_ml = 0, bytes = 0;
   int max_chunks = 1, part_rows = 0, chunk = TOKEN_CHUNK_MAX;
+  bool cluster = false;
 };
 static AttendWorkspace attend_workspace(const turq_kv_cache* kc, int64_t n_tokens, int32_t n_seqs, int32_t n_q_heads, int64_t max_new,
                                         int64_t max_context) {
   AttendWorkspace w;
   const int64_t group = n_q_heads / kc->n_kv_heads, most = max_new < n_tokens ? max_new : n_tokens;
   if (group < 1 || group > TOKEN_ROWS) return w;
-  w.chunk = (int)plan_token_chunk((int64_t)n_seqs * kc->n_kv_heads, max_context, kc->sm_count);
-  w.max_chunks = max_context <= w.chunk ? 1 : (int)((max_context + w.chunk - 1) / w.chunk);
+  const TokenPlan p = plan_tokens((int64_t)n_seqs * kc->n_kv_heads, max_context, kc->sm_count);
+  w.chunk = (int)p.chunk;
+  w.max_chunks = (int)p.chunks;
+  w.cluster = p.cluster;
   w.part_rows = (int)(most * group < TOKEN_ROWS ? most * group : TOKEN_ROWS);
-  if (w.max_chunks == 1) return w;
+  if (w.max_chunks == 1 || w.cluster) return w;
   const size_t rows = (size_t)n_seqs * kc->n_kv_heads * w.max_chunks * w.part_rows;
   w.off_ml = rows * kc->head_dim * 4;
   w.bytes = w.off_ml + rows * 8;
@@ -97,6 +100,7 @@ int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void*
   a.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(dev_workspace) + w.off_ml);
   a.max_chunks = w.max_chunks;
   a.chunk = w.chunk;
+  a.cluster = w.cluster;
   a.part_rows = w.part_rows;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;

@@ -25,6 +25,7 @@ struct AttendArgs {
   float *part, *part_ml;  // pieces of rows on their way to the kernel that joins them
   int max_chunks, part_rows;
   int chunk;              // keys of a chunk of a single token's context
+  int cluster;            // the chunks of a context are one cluster
 };
 
 __device__ __forceinline__ void report(int* status, int code) { *reinterpret_cast<volatile int*>(status) = code; }

@@ -57,4 +57,21 @@ inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64
   return best;
 }
 
+// Chunks as one cluster, whose blocks join their pieces over shared memory: no workspace, no second launch. Up to eight while all
+// run at once anyway, up to sixteen while they also find an SM each (more are hard to place: 3 users at 4096 keys in clusters
+// of 16 18.7 us, joined by a launch 11.1). Measured in a captured graph / called one by one, us, one user, 8 heads of 128, cluster
+// against launch: 1024 keys 6.2 / - against 6.6 / -, 4096 keys 9.2 / 11.0 against 8.2 / 16.1 (the second launch and the workspace cost
+// the host 5); 8192 keys in chunks of 512 12.3 against 9.9, which is why a chunk may not be longer than 256 for it.
+constexpr int TOKEN_CLUSTER = 16, TOKEN_CLUSTER_KEYS = 256;
+struct TokenPlan { int64_t chunk, chunks; bool cluster; };
+inline TokenPlan plan_tokens(int64_t pairs, int64_t max_context, int sms) {
+  TokenPlan p;
+  const int64_t sixteenth = (max_context + TOKEN_CLUSTER * TOKEN_STEP - 1) / (TOKEN_CLUSTER * TOKEN_STEP) * TOKEN_STEP;
+  p.chunk = plan_token_chunk(pairs, max_context, sms);
+  if (sixteenth > p.chunk && sixteenth <= TOKEN_CLUSTER_KEYS && pairs * TOKEN_CLUSTER <= sms) p.chunk = sixteenth;
+  p.chunks = max_context <= p.chunk ? 1 : (max_context + p.chunk - 1) / p.chunk;
+  p.cluster = p.chunks > 1 && p.chunks <= TOKEN_CLUSTER && pairs * p.chunks <= (int64_t)(p.chunks <= 8 ? TOKEN_CTAS : 1) * sms;
+  return p;
+}
+
 }  // namespace turq

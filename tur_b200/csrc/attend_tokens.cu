@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
   const Span sp = span_of(a, seq);
   const int rows = (int)sp.n * a.group;
   if (sp.n <= 0 || sp.n * a.group > TOKEN_ROWS) return;  // none, or the other kernel's
-  if (lo >= sp.ctx && chunk > 0) return;
+  if (lo >= sp.ctx && chunk > 0 && !a.cluster) return;   // (a cluster's blocks stay: they meet at its barriers)
   const int keys = (int)max((int64_t)0, min((int64_t)a.chunk, sp.ctx - lo));  // of this chunk
   const int steps = (keys + KEYS - 1) / KEYS;
   __syncthreads();
@@ -394,6 +394,9 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
   const bool whole = sp.ctx <= a.chunk;
   const int64_t item = ((int64_t)seq * a.cache.n_heads + head) * a.max_chunks + chunk;
   const float* const rb = reinterpret_cast<const float*>(raw + (base - s_u32(raw)));
+  // where a cluster's blocks leave their piece for one another: row r behind the result of warp r % 4
+  const uint32_t left = base + 16 * G::RES * 4 + 128;
+  static_assert(16 * G::RES * 4 + 128 + 4 * D * 4 + 32 <= G::RING, "a quarter of the piece's rows fits behind a warp's result");
   for (int i = threadIdx.x; i < rows * (D / 2); i += 32 * TOK_WARPS) {
     const int r = i / (D / 2), d = 2 * (i % (D / 2));
     float mm = -INFINITY, ll = 0.f, x = 0.f, y = 0.f;
@@ -408,15 +411,53 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
       x += f * v.x;
       y += f * v.y;
     }
-    if (whole) {
+    if (whole && chunk == 0) {
       const float inv = ll > 0.f ? 1.f / ll : ll == 0.f ? 0.f : ll;  // a row that sees no key gives zeros; NaN stays
       const int t = r / a.group, h = head * a.group + r % a.group;
       store_out2(a.out, a.out_dtype, ((sp.first + t) * a.hq + h) * D + d, x * inv, y * inv);
+    } else if (a.cluster) {
+      const uint32_t q = left + (r & 3) * G::RING;
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(q + ((r >> 2) * D + d) * 4), "f"(x), "f"(y) : "memory");
+      if (d == 0) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(q + 4 * D * 4 + (r >> 2) * 8), "f"(mm), "f"(ll) : "memory");
     } else {
       *reinterpret_cast<float2*>(a.part + (item * a.part_rows + r) * D + d) = make_float2(x, y);
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (item * a.part_rows + r) * 2) = make_float2(mm, ll);
     }
   }
+  if (!a.cluster) return;
+  // All chunks of the context are one cluster: its blocks read one another's pieces, each its share of the elements, and add them
+  // in chunk order.
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (!whole) {
+    const int chunks = (int)((sp.ctx + a.chunk - 1) / a.chunk);
+    for (int i = chunk * 32 * TOK_WARPS + threadIdx.x; i < rows * (D / 2); i += a.max_chunks * 32 * TOK_WARPS) {
+      const int r = i / (D / 2), d = 2 * (i % (D / 2));
+      const uint32_t q = left + (r & 3) * G::RING, qo = q + ((r >> 2) * D + d) * 4, qm = q + 4 * D * 4 + (r >> 2) * 8;
+      float2 ml[TOKEN_CLUSTER], v[TOKEN_CLUSTER];
+      float mm = -INFINITY, ll = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int k = 0; k < TOKEN_CLUSTER; k++) {
+        if (k >= chunks) break;
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[k].x), "=f"(ml[k].y) : "r"(map_to_rank(qm, k)));
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[k].x), "=f"(v[k].y) : "r"(map_to_rank(qo, k)));
+      }
+#pragma unroll
+      for (int k = 0; k < TOKEN_CLUSTER; k++)
+        if (k < chunks) mm = fmaxf(mm, ml[k].x);
+#pragma unroll
+      for (int k = 0; k < TOKEN_CLUSTER; k++) {
+        if (k >= chunks) break;
+        const float f = mm == -INFINITY ? 0.f : ex2(ml[k].x - mm);
+        ll += f * ml[k].y;
+        x += f * v[k].x;
+        y += f * v[k].y;
+      }
+      const float inv = ll > 0.f ? 1.f / ll : ll == 0.f ? 0.f : ll;
+      const int t = r / a.group, h = head * a.group + r % a.group;
+      store_out2(a.out, a.out_dtype, ((sp.first + t) * a.hq + h) * D + d, x * inv, y * inv);
+    }
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // nobody leaves while its piece is read
 }
 
 // The pieces of a row, in chunk order: a CTA per row, whose warps take every eighth piece and are added in their order. Its lanes
@@ -483,14 +524,15 @@ static cudaError_t launch_tokens_rows(const turq_kv_cache* kc, const AttendArgs&
   if (e != cudaSuccess) return e;
   if (!configured.done(dev)) {
     e = cudaFuncSetAttribute(attend_tokens_kernel<D, Q8, BF, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attend_tokens_kernel<D, Q8, BF, NR>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     configured.set(dev);
   }
   const TokMaps maps{kc->k16, kc->v16, kc->ks16, kc->vs16};
   (*launches)++;
-  e = launch_pdl(attend_tokens_kernel<D, Q8, BF, NR>, dim3((unsigned)a.max_chunks, (unsigned)a.cache.n_heads, (unsigned)a.n_seqs), dim3(32 * TOK_WARPS), SMEM, s,
-                 maps, a);
-  if (e != cudaSuccess || a.max_chunks == 1) return e;
+  e = launch_pdl_cluster(attend_tokens_kernel<D, Q8, BF, NR>, a.cluster ? (unsigned)a.max_chunks : 0u,
+                         dim3((unsigned)a.max_chunks, (unsigned)a.cache.n_heads, (unsigned)a.n_seqs), dim3(32 * TOK_WARPS), SMEM, s, maps, a);
+  if (e != cudaSuccess || a.max_chunks == 1 || a.cluster) return e;
   (*launches)++;
   return launch_pdl(join_tokens_kernel<D>, dim3((unsigned)a.part_rows, (unsigned)a.cache.n_heads, (unsigned)a.n_seqs), dim3(256), 0, s, a);
 }
