@@ -11,26 +11,37 @@
 
 namespace turq {
 
-// The workspace: pieces of single tokens' rows, their maxima and sums.
+// The workspace: pieces of single tokens' rows with their maxima and sums, pieces of tiles.
 struct AttendWorkspace {
-  size_t off_ml = 0, bytes = 0;
+  size_t off_ml = 0, off_tiles = 0, bytes = 0;
   int max_chunks = 1, part_rows = 0, chunk = TOKEN_CHUNK_MAX;
-  bool cluster = false;
+  int64_t pieces = 0;
+  bool cluster = false, tokens = false, tiles = false;  // which kernels the call may need
 };
 static AttendWorkspace attend_workspace(const turq_kv_cache* kc, int64_t n_tokens, int32_t n_seqs, int32_t n_q_heads, int64_t max_new,
                                         int64_t max_context) {
   AttendWorkspace w;
   const int64_t group = n_q_heads / kc->n_kv_heads, most = max_new < n_tokens ? max_new : n_tokens;
-  if (group < 1 || group > TOKEN_ROWS) return w;
-  const TokenPlan p = plan_tokens((int64_t)n_seqs * kc->n_kv_heads, max_context, kc->sm_count);
-  w.chunk = (int)p.chunk;
-  w.max_chunks = (int)p.chunks;
-  w.cluster = p.cluster;
-  w.part_rows = (int)(most * group < TOKEN_ROWS ? most * group : TOKEN_ROWS);
-  if (w.max_chunks == 1 || w.cluster) return w;
-  const size_t rows = (size_t)n_seqs * kc->n_kv_heads * w.max_chunks * w.part_rows;
-  w.off_ml = rows * kc->head_dim * 4;
-  w.bytes = w.off_ml + rows * 8;
+  auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
+  if (group < 1 || group > TILE_ROWS / 2) return w;
+  w.tokens = group <= TOKEN_ROWS;
+  w.tiles = most * group > TOKEN_ROWS;
+  if (w.tokens) {
+    const TokenPlan p = plan_tokens((int64_t)n_seqs * kc->n_kv_heads, max_context, kc->sm_count);
+    w.chunk = (int)p.chunk;
+    w.max_chunks = (int)p.chunks;
+    w.cluster = p.cluster;
+    w.part_rows = (int)(w.tiles ? TOKEN_ROWS : most * group);
+    if (p.chunks > 1 && !p.cluster) {
+      const size_t rows = (size_t)n_seqs * kc->n_kv_heads * p.chunks * w.part_rows;
+      w.off_ml = up(rows * kc->head_dim * 4);
+      w.off_tiles = w.bytes = w.off_ml + up(rows * 8);
+    }
+  }
+  if (w.tiles) {
+    w.pieces = plan_tile_pieces(n_tokens, n_seqs, group, kc->n_kv_heads, max_context, kc->sm_count);
+    if (w.pieces > 0) w.bytes += 256 + (size_t)w.pieces * TILE_ROWS * (8 + 8 + (size_t)kc->head_dim * 4);
+  }
   return w;
 }
 
@@ -102,17 +113,29 @@ int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void*
   a.chunk = w.chunk;
   a.cluster = w.cluster;
   a.part_rows = w.part_rows;
+  a.tile_pieces = (int)w.pieces;
+  a.sms = ctx->sm_count;
+  if (w.pieces > 0) {
+    uint8_t* const t = static_cast<uint8_t*>(dev_workspace) + w.off_tiles;
+    a.tile_head = reinterpret_cast<int*>(t);
+    a.tile_rows = reinterpret_cast<int64_t*>(t + 256);
+    a.tile_ml = reinterpret_cast<float2*>(t + 256 + w.pieces * turq::TILE_ROWS * 8);
+    a.tile_part = reinterpret_cast<float*>(t + 256 + w.pieces * turq::TILE_ROWS * 16);
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  const int64_t most = max_new < n_tokens ? max_new : n_tokens;
   int launches = 0;
-  if (most * a.group > turq::TOKEN_ROWS) {
-    const int64_t per_tile = 2 * (128 / a.group);  // tokens
-    const int64_t tiles = n_tokens / per_tile + n_seqs;  // no fewer than there are
-    if (tiles * hkv > INT32_MAX) return api_fail(ctx, TURQ_E_LIMIT, "more row tiles than a launch takes");
-    e = turq::launch_attend_tiles(cache, a, tiles, 1, s, &launches);
+  if (w.tiles) {
+    int64_t blocks = turq::tile_blocks(n_tokens, n_seqs, a.group, hkv);
+    if (blocks < w.pieces) blocks = w.pieces;
+    if (blocks > INT32_MAX) return api_fail(ctx, TURQ_E_LIMIT, "more row tiles than a launch takes");
+    e = turq::launch_attend_tiles(cache, a, (unsigned)blocks, s, &launches);
   }
-  if (e == cudaSuccess && a.group <= turq::TOKEN_ROWS) e = turq::launch_attend_tokens(cache, a, s, &launches);
+  if (e == cudaSuccess && w.tokens) {
+    a.beside = w.tiles;
+    e = turq::launch_attend_tokens(cache, a, s, &launches);
+  }
+  if (e == cudaSuccess && w.pieces > 0) e = turq::launch_join_tiles(cache, a, s, &launches);
   ctx->launches += launches;
   if (e != cudaSuccess) return turq::api_cuda_fail(ctx, e, "attention launch");
   return TURQ_OK;

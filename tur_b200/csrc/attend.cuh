@@ -26,6 +26,13 @@ struct AttendArgs {
   int max_chunks, part_rows;
   int chunk;              // keys of a chunk of a single token's context
   int cluster;            // the chunks of a context are one cluster
+  int beside;             // the tokens' launch runs beside the tiles' and need not wait for it before it ends
+  // tiles of rows: room for that many pieces (0: no row's keys are cut), their header, maxima and sums, sums, and the rows' places in out
+  int tile_pieces, sms;
+  int* tile_head;
+  float2* tile_ml;
+  float* tile_part;
+  int64_t* tile_rows;
 };
 
 __device__ __forceinline__ void report(int* status, int code) { *reinterpret_cast<volatile int*>(status) = code; }

@@ -74,4 +74,30 @@ inline TokenPlan plan_tokens(int64_t pairs, int64_t max_context, int sms) {
   return p;
 }
 
+// ---- tiles of rows: TILE_ROWS rows (two row tiles of the tensor core) a CTA, a CTA an SM
+constexpr int TILE_ROWS = 256;
+constexpr int TILE_SPLITS = 32;     // pieces of a tile's keys that the join takes
+constexpr int TILE_OVERHEAD = 4;    // what a CTA costs beside its key tiles, and what the join does, in key tiles of 128
+constexpr int TILE_WAVES = 3;       // pieces are no more than that many CTAs an SM
+// What cutting the keys of each of `ctas` tiles (the longest with `iters` key tiles) into s pieces costs: waves x (key tiles + overhead).
+// The kernel takes the s that costs least.
+TQ_HD int64_t tile_split_cost(int s, int ctas, int iters, int pieces, int sms) {
+  if (s > 1 && ((int64_t)s * ctas > pieces || 2 * s > iters)) return INT32_MAX;
+  return (int64_t)((s * ctas + sms - 1) / sms) * ((iters + s - 1) / s + TILE_OVERHEAD) + (s > 1 ? TILE_OVERHEAD : 0);
+}
+// Pairs of row tiles x key heads that a call has at most (floor(n / p) + sequences is no less than the sum of ceil(n_i / p)).
+inline int64_t tile_blocks(int64_t n_tokens, int64_t n_seqs, int64_t group, int64_t heads) {
+  const int64_t per_cta = TILE_ROWS / 2 / group * 2;  // tokens
+  return (n_seqs == 1 ? (n_tokens + per_cta - 1) / per_cta : n_tokens / per_cta + n_seqs) * heads;
+}
+// Pieces that a call gets room for: none where its tokens make more tiles than cutting could gain from.
+inline int64_t plan_tile_pieces(int64_t n_tokens, int64_t n_seqs, int64_t group, int64_t heads, int64_t max_context, int sms) {
+  const int64_t full = n_tokens / (TILE_ROWS / 2 / group * 2) * heads;  // tiles that are full, if all tokens are one sequence's
+  int64_t each = (max_context + 127) / 128 / 2;
+  if (each > TILE_SPLITS) each = TILE_SPLITS;
+  if (2 * full > TILE_WAVES * sms || each < 2) return 0;
+  const int64_t most = tile_blocks(n_tokens, n_seqs, group, heads) * each;
+  return most < TILE_WAVES * sms ? most : TILE_WAVES * sms;
+}
+
 }  // namespace turq

@@ -21,6 +21,7 @@
 namespace turq {
 
 constexpr int TILE_M = 128, TILE_N = 128;
+constexpr int POLY_OF = 8;
 
 template <int D, bool Q8> struct TileGeomA {
   static constexpr int HALVES = D / 64;
@@ -80,6 +81,47 @@ __device__ __forceinline__ void tile_box2(uint32_t dst, const CUtensorMap* map, 
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// The largest of three, one instruction.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two f32 at a time, one instruction.
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two f32 on the FMA units: x = n + f with n the nearest whole number (Cody and Waite; adding 1.5 x 2^23 rounds), 2^f by the
+// polynomial of degree 3 that is off by least, relative, on [-1/2, 1/2] (2^-13.7; fitted by Remez' exchange), n into the exponent.
+// Below 2^-126 it stays there: what comes of -inf is not quite zero.
+__device__ __forceinline__ void ex2_pair(uint64_t v, float& x, float& y) {
+  un2(v, x, y);
+  const uint64_t big = f2(12582912.f, 12582912.f), less = f2(-12582912.f, -12582912.f), one = f2(-1.f, -1.f);
+  v = f2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t t = add2(v, big);
+  const uint64_t f = fma2(add2(t, less), one, v);
+  uint64_t p = fma2(f, f2(0.05517166852951050f, 0.05517166852951050f), f2(0.2426111251115799f, 0.2426111251115799f));
+  p = fma2(p, f, f2(0.6932609677314758f, 0.6932609677314758f));
+  p = fma2(p, f, f2(0.9999280571937561f, 0.9999280571937561f));
+  float tx, ty;
+  un2(t, tx, ty);
+  un2(p, x, y);
+  x = __int_as_float(__float_as_int(x) + (__float_as_int(tx) << 23));
+  y = __int_as_float(__float_as_int(y) + (__float_as_int(ty) << 23));
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack_p(float a, float b) {
   if (BF) {
@@ -105,55 +147,92 @@ __device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volati
   __syncwarp();  // what follows is done by the warp as one
 }
 
+// The 128 threads of a row tile's softmax.
+__device__ __forceinline__ void tile_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+
 struct TileMaps { CUtensorMap k, v, ks, vs; };
 
 struct Work {
   Span sp;
   int seq, head, tok0, live;     // first new token of the CTA; whether there is any work
-  int id;                        // (list index x heads + head), for pieces
+  int id, split, splits;         // (index of the tile among those of the call) x heads + head; which piece of its keys
   int begin, end;                // key tiles
 };
 
-// The blockIdx.x / heads-th tile of the call, a sequence's last (longest) first.
-__device__ __forceinline__ void find_work(const AttendArgs& a, int tokens_per_cta, int splits, Work* w, int lane) {
-  int want = (int)(blockIdx.x / a.cache.n_heads);
-  const int head = (int)(blockIdx.x % a.cache.n_heads);
+// What a sequence asks of this kernel: pairs of row tiles, and the most key tiles of one.
+struct Ask { int tiles, iters; };
+__device__ __forceinline__ Ask ask_of(const AttendArgs& a, const Span& sp, int tokens_per_cta) {
+  Ask k{0, 0};
+  if (sp.n * a.group > TOKEN_ROWS) {
+    k.tiles = ((int)sp.n + tokens_per_cta - 1) / tokens_per_cta;
+    k.iters = ((int)sp.ctx + TILE_N - 1) / TILE_N;
+  }
+  return k;
+}
+
+// Block b takes piece b % splits of tile b / splits, a sequence's last (longest) tiles first. How many pieces follows from the tiles
+// that there really are, the same for every block. One warp.
+__device__ __forceinline__ void find_work(const AttendArgs& a, int tokens_per_cta, Work* w, int lane) {
   if (lane == 0) w->live = 0;
-  __syncwarp();
+  int total = 0, iters = 0;
+  Span sp{};
+  Ask ask{0, 0};
   for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-    Span sp{};
-    int tiles = 0;
+    ask = Ask{0, 0};
     if (s0 + lane < a.n_seqs) {
       sp = span_of(a, s0 + lane);
-      if (sp.n * a.group > TOKEN_ROWS) tiles = (int)((sp.n + tokens_per_cta - 1) / tokens_per_cta);
+      ask = ask_of(a, sp, tokens_per_cta);
     }
-    int upto = tiles;
+    total += __reduce_add_sync(0xFFFFFFFFu, ask.tiles);
+    iters = max(iters, __reduce_max_sync(0xFFFFFFFFu, ask.iters));
+  }
+  const int heads = a.cache.n_heads, ctas = total * heads;
+  // (lane i asks for i + 1 pieces)
+  const uint32_t mine = (uint32_t)min(tile_split_cost(lane + 1, ctas, iters, a.tile_pieces, a.sms), (int64_t)0x3FFFFFF) << 5 | (uint32_t)lane;
+  const int splits = (int)(__reduce_min_sync(0xFFFFFFFFu, mine) & 31u) + 1;
+  if (a.tile_pieces > 0 && blockIdx.x == 0 && lane == 0) {
+    a.tile_head[0] = splits;
+    a.tile_head[1] = ctas;
+  }
+  const int id = (int)blockIdx.x / splits;
+  if (id >= ctas) return;
+  int want = id / heads;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+    if (a.n_seqs > 32) {  // (up to 32: still in registers)
+      ask = Ask{0, 0};
+      if (s0 + lane < a.n_seqs) {
+        sp = span_of(a, s0 + lane);
+        ask = ask_of(a, sp, tokens_per_cta);
+      }
+    }
+    int upto = ask.tiles;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int t = __shfl_up_sync(0xFFFFFFFFu, upto, d);
       if (lane >= d) upto += t;
     }
-    const int total = __shfl_sync(0xFFFFFFFFu, upto, 31);
-    if (want < total) {
-      if (want < upto && want >= upto - tiles) {
-        const int tile = tiles - 1 - (want - (upto - tiles));
+    const int here = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (want < here) {
+      if (want < upto && want >= upto - ask.tiles) {
+        const int tile = ask.tiles - 1 - (want - (upto - ask.tiles));
         w->sp = sp;
         w->seq = s0 + lane;
-        w->head = head;
+        w->head = id % heads;
         w->tok0 = tile * tokens_per_cta;
-        w->id = (int)blockIdx.x;
+        w->id = id;
+        w->split = (int)blockIdx.x % splits;
+        w->splits = splits;
         const int64_t last = min(sp.n, (int64_t)w->tok0 + tokens_per_cta) - 1;
         const int keys = (int)min(sp.ctx, keys_seen(sp, last, a.causal));
         const int n = (keys + TILE_N - 1) / TILE_N;
-        w->begin = (int)((int64_t)n * blockIdx.y / splits);
-        w->end = (int)((int64_t)n * (blockIdx.y + 1) / splits);
+        w->begin = n * w->split / splits;  // (32 bits hold 2^23 key tiles x 32)
+        w->end = n * (w->split + 1) / splits;
         w->live = 1;
       }
-      break;
+      return;
     }
-    want -= total;
+    want -= here;
   }
-  __syncwarp();
 }
 
 template <int D, bool Q8, bool BF>
@@ -161,82 +240,102 @@ __global__ void __launch_bounds__((TileGeomA<D, Q8>::THREADS), 1)
 attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ AttendArgs a) {
   using G = TileGeomA<D, Q8>;
   constexpr int ST = G::STAGES, OP = G::OPERAND, HB = TILE_N * 128;  // HB: one 64-column block
-  constexpr uint32_t COL_S = 0, COL_O = 256;                          // S (and P) of tile t at 128 t, O at 256 + D t
+  constexpr int POLY = D == 128 ? 0 : 1;
+  constexpr bool APART = D == 64;                                     // P has columns of its own: S may be written again once it is read
+  constexpr uint32_t COL_S = 0, COL_O = 256, COL_P = APART ? 384 : 0;                          // S of tile t at 128 t, O at 256 + D t, P at 384 + 64 t or where S was
   extern __shared__ uint8_t raw[];
-  __shared__ __align__(8) uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], p_full[2], o_full, v_fixed, raw_full[3], raw_empty[3];
+  __shared__ __align__(8) uint64_t q_full[2], kv_full[8], kv_empty[8], s_full[2], p_full[2][2], s_read[2], o_full[2], v_fixed, raw_full[3], raw_empty[3];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ Work work;
+  __shared__ float row_up[2][TILE_M];  // the power of two that a row of Q was divided by
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (s_u32(raw) + 1023u) & ~1023u;
   const uint32_t sQ = smem, sKV = smem + 2 * OP, sRaw = sKV + ST * OP;
   volatile int* const abort_flag = &abort_word;
   const int tpt = TILE_M / a.group;  // tokens of a tile
 
-  if (warp == 0) find_work(a, 2 * tpt, (int)gridDim.y, &work, lane);
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&tmem_slot)), "n"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   if (threadIdx.x == 32) {
-    for (int i = 0; i < 2; i++) { bar_init(&q_full[i], 4); bar_init(&s_full[i], 1); bar_init(&p_full[i], 4); }
+    for (int i = 0; i < 2; i++) { bar_init(&q_full[i], 4); bar_init(&s_full[i], 1); bar_init(&p_full[i][0], 4); bar_init(&p_full[i][1], 4); bar_init(&s_read[i], 4); bar_init(&o_full[i], 1); }
     for (int i = 0; i < ST; i++) { bar_init(&kv_full[i], Q8 ? 4 : 1); bar_init(&kv_empty[i], 1); }
-    bar_init(&o_full, 1);
     bar_init(&v_fixed, 1);
     for (int i = 0; i < 3; i++) { bar_init(&raw_full[i], 1); bar_init(&raw_empty[i], 4); }
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-  if (!work.live) return;
-  const Span sp = work.sp;
-  const int seq = work.seq, head = work.head, begin = work.begin, n_iter = work.end - work.begin;
-  const int tiles = sp.n - work.tok0 > tpt ? 2 : 1;  // row tiles with rows
-  const int ctx = (int)sp.ctx;
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&tmem_slot)), "n"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if (threadIdx.x == 288) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
   }
+  // launched behind its predecessor's last block: everything that kernels before it wrote is read from here on
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp == 0) find_work(a, 2 * tpt, &work, lane);
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = tmem_slot;
+  if (!work.live) {
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    return;
+  }
+  const Span sp = work.sp;
+  const int seq = work.seq, head = work.head, begin = work.begin, n_iter = work.end - work.begin;
+  const int tiles = sp.n - work.tok0 > tpt ? 2 : 1;  // row tiles with rows
+  const int ctx = (int)sp.ctx;
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::REG_SOFT));
     const int t = warp >> 2, r = threadIdx.x & 127;
-    const int tok = work.tok0 + t * tpt + r / a.group;
+    const uint32_t per16 = 65535u / (uint32_t)a.group + 1u;              // row / group = row x per16 >> 16 for rows and groups up to 128
+    const int tok = work.tok0 + t * tpt + (int)((r * per16) >> 16);
     const bool live = r < tpt * a.group && tok < sp.n;
-    const int qh = head * a.group + r % a.group;
     float mul = a.scale_log2;
-    // Q into the operand layout; on f16 caches a bf16 row by the power of two that its largest element fits
+    // Q into the operand layout, D / 8 lanes a row (a row a thread, every load would touch 32 lines: 7500 cycles against 1500); on f16
+    // caches a bf16 row by the power of two that its largest element fits.
     if (t < tiles) {
-      const uint4* qp = reinterpret_cast<const uint4*>(a.q + (sp.first + (live ? tok : 0)) * a.q_stride + (int64_t)qh * D);
+      constexpr int L = D / 8, ROWS = TILE_M / L;  // rows of a pass
+      const int ch = r % L;
+      uint4 w[L];
+#pragma unroll
+      for (int i = 0; i < L; i++) {
+        const int row = i * ROWS + r / L, rt = (int)((row * per16) >> 16), tk = work.tok0 + t * tpt + rt;
+        const bool ok = row < tpt * a.group && tk < sp.n;
+        w[i] = ok ? *(reinterpret_cast<const uint4*>(a.q + (sp.first + tk) * a.q_stride + (int64_t)(head * a.group + row - rt * a.group) * D) + ch)
+                  : make_uint4(0, 0, 0, 0);
+      }
       const bool convert = !BF && a.q_bf16;
-      float down = 1.f;
-      if (convert) {
-        uint32_t top = 0;
-        for (int i = 0; i < D / 8; i++) {
-          const uint4 w = live ? qp[i] : make_uint4(0, 0, 0, 0);
-          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < L; i++) {
+        const int row = i * ROWS + r / L;
+        if (convert) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(&w[i]);
+          uint32_t top = 0;
 #pragma unroll
           for (int e = 0; e < 4; e++) top = max(top, max(x[e] & 0x7FFFu, (x[e] >> 16) & 0x7FFFu));
-        }
-        const int e = min(max((int)(top >> 7) - 127, -100), 100);
-        down = __uint_as_float((uint32_t)(127 - e) << 23);
-        mul *= __uint_as_float((uint32_t)(127 + e) << 23);
-      }
-#pragma unroll 4
-      for (int i = 0; i < D / 8; i++) {
-        uint4 w = live ? qp[i] : make_uint4(0, 0, 0, 0);
-        if (convert) {
-          uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+          for (int d = 1; d < L; d <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+          const int e2 = min(max((int)(top >> 7) - 127, -100), 100);
+          const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+          if (ch == 0) row_up[t][row] = __uint_as_float((uint32_t)(127 + e2) << 23);
 #pragma unroll
           for (int e = 0; e < 4; e++) x[e] = pack_p<false>(__uint_as_float(x[e] << 16) * down, __uint_as_float(x[e] & 0xFFFF0000u) * down);
         }
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sQ + t * OP + (i >> 3) * HB + r * 128 + (((i & 7) ^ (r & 7)) << 4)), "r"(w.x), "r"(w.y),
-                     "r"(w.z), "r"(w.w) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sQ + t * OP + (ch >> 3) * HB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)), "r"(w[i].x),
+                     "r"(w[i].y), "r"(w[i].z), "r"(w[i].w) : "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) bar_arrive(&q_full[t]);
+      if (convert) {
+        tile_sync(1 + t);
+        mul *= row_up[t][r];
+      }
     }
     const int seen = live ? (int)min(sp.ctx, keys_seen(sp, tok, a.causal)) : INT32_MAX;  // rows that do not exist ask for no mask
     // keys that every row of the warp sees
@@ -244,33 +343,51 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, d));
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in the address' upper half
-    const uint32_t tS = tmem + lanes + COL_S + 128 * t, tO = tmem + lanes + COL_O + D * t;
+    const uint32_t tS = tmem + lanes + COL_S + 128 * t, tO = tmem + lanes + COL_O + D * t, tP = APART ? tmem + lanes + COL_P + 64 * t : tS;
     float m = -INFINITY, l = 0.f;  // maximum in units of S, as last subtracted; sum of the weights
     const float lag = 8.f / mul;
+    if (t >= tiles && work.splits > 1 && work.split == 0) a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = -1;
     if (t < tiles) {
       for (int j = 0; j < n_iter; j++) {
         float s[TILE_N];
         tile_wait(&s_full[t], j & 1, abort_flag);
         tc_after();
-#pragma unroll
-        for (int i = 0; i < 4; i++) tmem_ld32(s + 32 * i, tS + 32 * i);
+        tmem_ld32(s, tS);
+        tmem_ld32(s + 32, tS + 32);
         tmem_wait_ld();
+        tmem_ld32(s + 64, tS + 64);
+        tmem_ld32(s + 96, tS + 96);
         const int k0 = (begin + j) * TILE_N;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto largest = [&](int from) {
+#pragma unroll
+          for (int i = from; i < from + 64; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) top[e] = max3(top[e], s[i + 2 * e], s[i + 2 * e + 1]);
+          }
+        };
         if (k0 + TILE_N > least) {
+          tmem_wait_ld();
           const int lim = seen - k0;
 #pragma unroll
           for (int i = 0; i < TILE_N; i++) s[i] = i < lim ? s[i] : -INFINITY;
         }
-        float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < TILE_N; i += 4) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], s[i + e]);
+        largest(0);
+        tmem_wait_ld();
+        if (APART) {  // all of S is in registers
+          tc_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&s_read[t]);
         }
-        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        largest(64);
+        const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]);
         if (j == 0) {
           m = mt;
         } else if (__any_sync(0xFFFFFFFFu, mt > m + lag)) {
+          if (APART) {  // otherwise a full S says so
+            tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
+            tc_after();
+          }
           const float m2 = fmaxf(m, mt), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * mul);  // m = -inf: 0 of nothing
           m = m2;
           l *= f;
@@ -286,38 +403,80 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           tmem_wait_st();
         }
         const float sub = m == -INFINITY ? 0.f : m * mul;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        if (APART && j > 0) {  // the last weights' product has read them
+          tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
+          tc_after();
+        }
+        const uint64_t mul2 = f2(mul, mul), sub2 = f2(-sub, -sub);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int h = 0; h < TILE_N / 32; h++) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            const float x = ex2(fmaf(s[32 * h + 2 * i], mul, -sub)), y = ex2(fmaf(s[32 * h + 2 * i + 1], mul, -sub));
-            sum[(2 * i) & 3] += x;
-            sum[(2 * i + 1) & 3] += y;
+            float x, y;
+            const uint64_t e = fma2(f2(s[32 * h + 2 * i], s[32 * h + 2 * i + 1]), mul2, sub2);
+            if (i % POLY_OF < POLY) {
+              ex2_pair(e, x, y);
+            } else {
+              un2(e, x, y);
+              x = ex2(x);
+              y = ex2(y);
+            }
+            sum[i & 1] = add2(sum[i & 1], f2(x, y));
             p[i] = pack_p<BF>(x, y);
           }
-          tmem_st16(tS + 16 * h, p);
+          tmem_st16(tP + 16 * h, p);
+          if (h % 2 == 1) {  // half of the weights: their product may start
+            tmem_wait_st();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&p_full[t][h / 2]);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(&p_full[t]);
+        float s0, s1;
+        un2(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
       }
+      if (m == -INFINITY) l = 0.f;  // a row that saw no key
       if (n_iter > 0) {
-        tile_wait(&o_full, 0, abort_flag);
+        tile_wait(&o_full[t], APART ? (n_iter - 1) & 1 : 0, abort_flag);
         tc_after();
       }
-      const bool pieces = gridDim.y > 1;
+      const bool pieces = work.splits > 1;
       const float inv = pieces ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a row that sees no key gives zeros; NaN stays
-      const int64_t out = ((sp.first + tok) * a.hq + qh) * D;
-      const int64_t piece = ((int64_t)work.id * gridDim.y + blockIdx.y) * (2 * TILE_M) + TILE_M * t + r;
-      if (pieces) *reinterpret_cast<float2*>(a.part_ml + 2 * piece) = make_float2(m * mul, live ? l : 0.f);
-      const bool store = live && !*abort_flag;
+      const int64_t piece0 = (int64_t)blockIdx.x * (2 * TILE_M) + TILE_M * t;
+      if (pieces) {
+        a.tile_ml[piece0 + r] = make_float2(m * mul, l);
+        if (work.split == 0) {
+          const int64_t out = ((work.sp.first + tok) * a.hq + work.head * a.group + r - (int)((r * per16) >> 16) * a.group) * D;
+          a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = live ? out : -1;
+        }
+      }
+      // Rows go out through shared memory, a warp whole rows, for the same reason as Q comes in so (6500 cycles against 1500): through this
+      // tile's part of Q, which nothing reads any more, in one go or in two for 32 bits.
+      const bool wide = pieces || a.out_dtype == TURQ_F32;
+      const uint32_t stage = sQ + t * OP;
+      constexpr int L = D / 8;  // 16-byte chunks of a staged row
+      uint8_t* const to = static_cast<uint8_t*>(pieces ? static_cast<void*>(a.tile_part) : a.out);
+      const bool store = !*abort_flag;
+      auto flush = [&](int pass) {
+        tile_sync(1 + t);
+#pragma unroll 4
+        for (int i = 0; i < L; i++) {
+          const int row = i * (TILE_M / L) + r / L, ch = r % L, rt = (int)((row * per16) >> 16), tk = work.tok0 + t * tpt + rt;
+          if (row < tpt * a.group && tk < work.sp.n && store) {
+            uint4 w;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(stage + row * 2 * D + ((ch ^ (row & 7)) << 4)));
+            const int64_t at = (pieces ? piece0 + row : (work.sp.first + tk) * a.hq + work.head * a.group + row - rt * a.group) * D;
+            *reinterpret_cast<uint4*>(to + at * (wide ? 4 : 2) + pass * 2 * D + 16 * ch) = w;
+          }
+        }
+        tile_sync(1 + t);
+      };
+#pragma unroll 1
       for (int i = 0; i < D / 32; i++) {
         float o[32];
-        __syncwarp();
         if (n_iter > 0) {
           tmem_ld32(o, tO + 32 * i);
           tmem_wait_ld();
@@ -325,27 +484,28 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 32; e++) o[e] = 0.f;
         }
-        if (!store) {
-        } else if (pieces) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(a.part + piece * D + 32 * i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        } else if (a.out_dtype == TURQ_F32) {
+        for (int e = 0; e < 32; e++) o[e] *= inv;
+        if (wide) {
+          const int c = i % (D / 64);
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + out + 32 * i + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+            asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(stage + r * 2 * D + (((8 * c + e / 4) ^ (r & 7)) << 4)), "f"(o[e]), "f"(o[e + 1]),
+                         "f"(o[e + 2]), "f"(o[e + 3]) : "memory");
+          if (c == D / 64 - 1) flush(i / (D / 64));
         } else {
           const bool bf = a.out_dtype == TURQ_BF16;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint32_t w[4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-              const float x = o[e + 2 * q] * inv, y = o[e + 2 * q + 1] * inv;
-              w[q] = bf ? pack_p<true>(x, y) : pack_p<false>(x, y);
-            }
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + out + 32 * i + e) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int q = 0; q < 4; q++) w[q] = bf ? pack_p<true>(o[e + 2 * q], o[e + 2 * q + 1]) : pack_p<false>(o[e + 2 * q], o[e + 2 * q + 1]);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + r * 2 * D + (((4 * i + e / 8) ^ (r & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                         "r"(w[3]) : "memory");
           }
+          if (i == D / 32 - 1) flush(0);
         }
+        __syncwarp();
       }
     }
   } else {
@@ -369,11 +529,11 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         }
         tc_commit(&s_full[t]);
       };
-      auto pv = [&](int t, int stage, bool first) {
+      auto pv = [&](int t, int stage, int half, bool first) {
         if (!issuer) return;
 #pragma unroll
-        for (int i = 0; i < TILE_N / 16; i++)
-          mma_ts(tmem + COL_O + D * t, tmem + COL_S + 128 * t + 8 * i, v_hi | (uint64_t)(kv_lo + stage * (OP >> 4) + 128 * i), id_pv, !first || i > 0);
+        for (int i = TILE_N / 32 * half; i < TILE_N / 32 * (half + 1); i++)
+          mma_ts(tmem + COL_O + D * t, tmem + (APART ? COL_P + 64 * t : COL_S + 128 * t) + 8 * i, v_hi | (uint64_t)(kv_lo + stage * (OP >> 4) + 128 * i), id_pv, !first || i > 0);
       };
       if (n_iter > 0) {
         int ks = 0, vs = 1 % ST;  // stages: K_0, V_0, K_1, V_1, ...
@@ -391,14 +551,29 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         for (int j = 0; j < n_iter; j++) {
           if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
           const bool more = j + 1 < n_iter;
-          tile_wait(&kv_full[vs], vp, abort_flag);
-          if (!Q8 && (begin + j + 1) * TILE_N > ctx) tile_wait(&v_fixed, 0, abort_flag);
+          if (!APART) tile_wait(&kv_full[vs], vp, abort_flag);
+          if (!APART && !Q8 && (begin + j + 1) * TILE_N > ctx) tile_wait(&v_fixed, 0, abort_flag);
+          if (APART && more) {  // the next S as soon as the last is read
+            tile_wait(&kv_full[ks], kp, abort_flag);
+            for (int t = 0; t < tiles; t++) {
+              tile_wait(&s_read[t], j & 1, abort_flag);
+              tc_after();
+              qk(t, ks);
+            }
+            if (issuer) tc_commit(&kv_empty[ks]);
+          }
+          if (APART) tile_wait(&kv_full[vs], vp, abort_flag);
+          if (APART && !Q8 && (begin + j + 1) * TILE_N > ctx) tile_wait(&v_fixed, 0, abort_flag);
           for (int t = 0; t < tiles; t++) {
-            tile_wait(&p_full[t], j & 1, abort_flag);
-            tc_after();
-            pv(t, vs, j == 0);
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              tile_wait(&p_full[t][half], j & 1, abort_flag);
+              tc_after();
+              pv(t, vs, half, j == 0);
+            }
+            if (issuer && (APART || !more)) tc_commit(&o_full[t]);
             if (t == tiles - 1 && issuer) tc_commit(&kv_empty[vs]);
-            if (more) {
+            if (!APART && more) {
               if (t == 0) {
                 tile_wait(&kv_full[ks], kp, abort_flag);
                 tc_after();
@@ -410,7 +585,6 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           next(vs, vp);
           next(ks, kp);
         }
-        if (issuer) tc_commit(&o_full);
       }
       __syncwarp();
     } else if (warp == 9) {
@@ -532,8 +706,46 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
   }
 }
 
+// The pieces of rows whose keys were cut, in their order: a warp per row, 32 rows a block.
+template <int D>
+__global__ void __launch_bounds__(256) join_tiles_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int E = D / 32;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int splits = a.tile_head[0], lane = threadIdx.x & 31;
+  if (splits <= 1 || (int)blockIdx.x >= a.tile_head[1]) return;
+  for (int i = 0; i < 4; i++) {
+    const int r = blockIdx.y * 32 + (threadIdx.x >> 5) * 4 + i;
+    const int64_t out = a.tile_rows[(int64_t)blockIdx.x * (2 * TILE_M) + r];
+    if (out < 0) continue;
+    const int64_t piece = (int64_t)blockIdx.x * splits * (2 * TILE_M) + r;
+    float mm = -INFINITY, ll = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.f;
+    const float2 mine = lane < splits ? a.tile_ml[piece + (int64_t)lane * (2 * TILE_M)] : make_float2(-INFINITY, 0.f);  // at most 32 of them
+    mm = mine.x;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, d));
+    const float f = mm == -INFINITY ? 0.f : ex2(mine.x - mm), fl = f * mine.y;
+#pragma unroll 4
+    for (int k = 0; k < splits; k++) {
+      const float w = __shfl_sync(0xFFFFFFFFu, f, k);
+      const float* p = a.tile_part + (piece + (int64_t)k * (2 * TILE_M)) * D + lane * E;
+      ll += __shfl_sync(0xFFFFFFFFu, fl, k);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(p + e);
+        o[e] += w * v.x;
+        o[e + 1] += w * v.y;
+      }
+    }
+    const float inv = ll > 0.f ? 1.f / ll : ll == 0.f ? 0.f : ll;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) store_out2(a.out, a.out_dtype, out + lane * E + e, o[e] * inv, o[e + 1] * inv);
+  }
+}
+
 template <int D, bool Q8, bool BF>
-static cudaError_t launch_tiles(const turq_kv_cache* kc, const AttendArgs& a, int64_t tiles, int splits, cudaStream_t s) {
+static cudaError_t launch_tiles(const turq_kv_cache* kc, const AttendArgs& a, unsigned blocks, cudaStream_t s) {
   using G = TileGeomA<D, Q8>;
   static PerDeviceOnce configured;
   int dev = 0;
@@ -545,18 +757,23 @@ static cudaError_t launch_tiles(const turq_kv_cache* kc, const AttendArgs& a, in
     configured.set(dev);
   }
   const TileMaps maps{kc->k_tile, kc->v_tile, kc->ks16, kc->vs16};
-  attend_tiles_kernel<D, Q8, BF><<<dim3((unsigned)(tiles * a.cache.n_heads), (unsigned)splits), G::THREADS, G::SMEM, s>>>(maps, a);
-  return cudaGetLastError();
+  return launch_pdl(attend_tiles_kernel<D, Q8, BF>, dim3(blocks), dim3(G::THREADS), G::SMEM, s, maps, a);
 }
 
-cudaError_t launch_attend_tiles(const turq_kv_cache* kc, const AttendArgs& a, int64_t tiles, int splits, cudaStream_t s, int* launches) {
+cudaError_t launch_attend_tiles(const turq_kv_cache* kc, const AttendArgs& a, unsigned blocks, cudaStream_t s, int* launches) {
   (*launches)++;
   if (kc->head_dim == 128) {
-    if (kc->dtype == TURQ_Q8_0) return launch_tiles<128, true, false>(kc, a, tiles, splits, s);
-    return kc->dtype == TURQ_BF16 ? launch_tiles<128, false, true>(kc, a, tiles, splits, s) : launch_tiles<128, false, false>(kc, a, tiles, splits, s);
+    if (kc->dtype == TURQ_Q8_0) return launch_tiles<128, true, false>(kc, a, blocks, s);
+    return kc->dtype == TURQ_BF16 ? launch_tiles<128, false, true>(kc, a, blocks, s) : launch_tiles<128, false, false>(kc, a, blocks, s);
   }
-  if (kc->dtype == TURQ_Q8_0) return launch_tiles<64, true, false>(kc, a, tiles, splits, s);
-  return kc->dtype == TURQ_BF16 ? launch_tiles<64, false, true>(kc, a, tiles, splits, s) : launch_tiles<64, false, false>(kc, a, tiles, splits, s);
+  if (kc->dtype == TURQ_Q8_0) return launch_tiles<64, true, false>(kc, a, blocks, s);
+  return kc->dtype == TURQ_BF16 ? launch_tiles<64, false, true>(kc, a, blocks, s) : launch_tiles<64, false, false>(kc, a, blocks, s);
+}
+
+cudaError_t launch_join_tiles(const turq_kv_cache* kc, const AttendArgs& a, cudaStream_t s, int* launches) {
+  (*launches)++;
+  const dim3 grid((unsigned)(a.tile_pieces / 2), 2 * TILE_M / 32);  // two pieces a tile at least
+  return kc->head_dim == 64 ? launch_pdl(join_tiles_kernel<64>, grid, dim3(256), 0, s, a) : launch_pdl(join_tiles_kernel<128>, grid, dim3(256), 0, s, a);
 }
 
 }  // namespace turq

@@ -104,16 +104,21 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
     for (int s = 0; s < TOK_STAGES; s++) bar_init(&full[warp][s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // launched behind its predecessor's last block: everything that kernels before it wrote is read from here on
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Launched behind its predecessor's last block: everything that kernels before it wrote is read from here on. Beside the tiles of the
+  // same call there is nothing to wait for (they started behind those kernels), but one block stays until they are done, so
+  // that whoever waits for this launch has waited for both.
+  if (!a.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // Pages of the chunk, 16 keys each, at the same time as the lengths: entries behind the context are dropped afterwards.
   const int shift = a.cache.page_shift, most = (int)min((int64_t)a.chunk, a.max_context - lo);
   for (int i = threadIdx.x; i < (most + 15) / 16; i += 32 * TOK_WARPS) pages[i] = a.page_table[seq * a.table_stride + ((lo + 16 * i) >> shift)];
   const Span sp = span_of(a, seq);
   const int rows = (int)sp.n * a.group;
-  if (sp.n <= 0 || sp.n * a.group > TOKEN_ROWS) return;  // none, or the other kernel's
-  if (lo >= sp.ctx && chunk > 0 && !a.cluster) return;   // (a cluster's blocks stay: they meet at its barriers)
+  auto leave = [&]() {
+    if (a.beside && threadIdx.x == 0 && (blockIdx.x | blockIdx.y | blockIdx.z) == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
+  if (sp.n <= 0 || sp.n * a.group > TOKEN_ROWS) return leave();  // none, or the other kernel's
+  if (lo >= sp.ctx && chunk > 0 && !a.cluster) return leave();   // (a cluster's blocks stay: they meet at its barriers)
   const int keys = (int)max((int64_t)0, min((int64_t)a.chunk, sp.ctx - lo));  // of this chunk
   const int steps = (keys + KEYS - 1) / KEYS;
   __syncthreads();
@@ -424,7 +429,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (item * a.part_rows + r) * 2) = make_float2(mm, ll);
     }
   }
-  if (!a.cluster) return;
+  if (!a.cluster) return leave();
   // All chunks of the context are one cluster: its blocks read one another's pieces, each its share of the elements, and add them
   // in chunk order.
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -458,6 +463,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
     }
   }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // nobody leaves while its piece is read
+  leave();
 }
 
 // The pieces of a row, in chunk order: a CTA per row, whose warps take every eighth piece and are added in their order. Its lanes
