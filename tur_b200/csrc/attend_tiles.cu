@@ -150,6 +150,9 @@ __device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, volati
 // The 128 threads of a row tile's softmax.
 __device__ __forceinline__ void tile_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 
+__device__ __forceinline__ void turn_wait(int id) { asm volatile("bar.sync %0, 256;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void turn_give(int id) { asm volatile("bar.arrive %0, 256;" ::"r"(id) : "memory"); }
+
 struct TileMaps { CUtensorMap k, v, ks, vs; };
 
 struct Work {
@@ -348,6 +351,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
     const float lag = 8.f / mul;
     if (t >= tiles && work.splits > 1 && work.split == 0) a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = -1;
     if (t < tiles) {
+      if (tiles == 2 && t == 1 && n_iter > 0) turn_give(3);
       for (int j = 0; j < n_iter; j++) {
         float s[TILE_N];
         tile_wait(&s_full[t], j & 1, abort_flag);
@@ -407,6 +411,9 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
           tc_after();
         }
+        // The tiles take turns at the exponentials, which one warp a scheduler can keep busy: together both would take as long as one behind
+        // the other, and then both wait for the tensor core at once.
+        if (tiles == 2) turn_wait(3 + t);
         const uint64_t mul2 = f2(mul, mul), sub2 = f2(-sub, -sub);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -437,6 +444,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         float s0, s1;
         un2(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
+        if (tiles == 2 && (t == 0 || j + 1 < n_iter)) turn_give(3 + (t ^ 1));
       }
       if (m == -INFINITY) l = 0.f;  // a row that saw no key
       if (n_iter > 0) {
