@@ -26,7 +26,7 @@ constexpr int POLY_OF = 8;
 template <int D, bool Q8> struct TileGeomA {
   static constexpr int HALVES = D / 64;
   static constexpr int OPERAND = TILE_N * D * 2;      // a tile of K, V or Q: blocks of 64 columns, 128 rows of 128 bytes each
-  static constexpr int STAGES = Q8 ? 3 : (D == 128 ? 5 : 8);
+  static constexpr int STAGES = Q8 ? 3 : (D == 128 ? 4 : 8);
   static constexpr int RAW = Q8 ? TILE_N * D + 1024 : 0;  // int8 rows, scales behind them
   static constexpr int RAW_STAGES = Q8 ? 3 : 0;
   static constexpr int THREADS = Q8 ? 512 : 384;
@@ -252,6 +252,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
   __shared__ int abort_word;
   __shared__ Work work;
   __shared__ float row_up[2][TILE_M];  // the power of two that a row of Q was divided by
+  __shared__ int row_at[2][TILE_M];    // a row's token (of the tile) and, above 8 bits, its head (of the group); -1: no such row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (s_u32(raw) + 1023u) & ~1023u;
   const uint32_t sQ = smem, sKV = smem + 2 * OP, sRaw = sKV + ST * OP;
@@ -295,22 +296,23 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
     // ---------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::REG_SOFT));
     const int t = warp >> 2, r = threadIdx.x & 127;
-    const uint32_t per16 = 65535u / (uint32_t)a.group + 1u;              // row / group = row x per16 >> 16 for rows and groups up to 128
-    const int tok = work.tok0 + t * tpt + (int)((r * per16) >> 16);
-    const bool live = r < tpt * a.group && tok < sp.n;
+    // row / group = row x per16 >> 16 for rows and groups up to 128
+    const int rt = (int)((r * (65535u / (uint32_t)a.group + 1u)) >> 16), tok = work.tok0 + t * tpt + rt;
+    const bool live = rt < tpt && tok < sp.n;
+    row_at[t][r] = live ? rt | (r - rt * a.group) << 8 : -1;  // once, and not for every 16 bytes that come or go
+    tile_sync(1 + t);
     float mul = a.scale_log2;
     // Q into the operand layout, D / 8 lanes a row (a row a thread, every load would touch 32 lines: 7500 cycles against 1500); on f16
     // caches a bf16 row by the power of two that its largest element fits.
     if (t < tiles) {
       constexpr int L = D / 8, ROWS = TILE_M / L;  // rows of a pass
       const int ch = r % L;
+      const uint16_t* const qp = a.q + (sp.first + work.tok0 + t * tpt) * a.q_stride + (int64_t)head * a.group * D + 8 * ch;
       uint4 w[L];
 #pragma unroll
       for (int i = 0; i < L; i++) {
-        const int row = i * ROWS + r / L, rt = (int)((row * per16) >> 16), tk = work.tok0 + t * tpt + rt;
-        const bool ok = row < tpt * a.group && tk < sp.n;
-        w[i] = ok ? *(reinterpret_cast<const uint4*>(a.q + (sp.first + tk) * a.q_stride + (int64_t)(head * a.group + row - rt * a.group) * D) + ch)
-                  : make_uint4(0, 0, 0, 0);
+        const int at = row_at[t][i * ROWS + r / L];
+        w[i] = at >= 0 ? *reinterpret_cast<const uint4*>(qp + (at & 255) * a.q_stride + (at >> 8) * D) : make_uint4(0, 0, 0, 0);
       }
       const bool convert = !BF && a.q_bf16;
 #pragma unroll
@@ -454,11 +456,12 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       const bool pieces = work.splits > 1;
       const float inv = pieces ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a row that sees no key gives zeros; NaN stays
       const int64_t piece0 = (int64_t)blockIdx.x * (2 * TILE_M) + TILE_M * t;
+      const int64_t out0 = ((work.sp.first + work.tok0 + t * tpt) * a.hq + work.head * a.group) * D;  // of the tile's first row
       if (pieces) {
         a.tile_ml[piece0 + r] = make_float2(m * mul, l);
         if (work.split == 0) {
-          const int64_t out = ((work.sp.first + tok) * a.hq + work.head * a.group + r - (int)((r * per16) >> 16) * a.group) * D;
-          a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = live ? out : -1;
+          const int at = row_at[t][r];
+          a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = at < 0 ? -1 : out0 + ((int64_t)(at & 255) * a.hq + (at >> 8)) * D;
         }
       }
       // Rows go out through shared memory, a warp whole rows, for the same reason as Q comes in so (6500 cycles against 1500): through this
@@ -466,19 +469,19 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       const bool wide = pieces || a.out_dtype == TURQ_F32;
       const uint32_t stage = sQ + t * OP;
       constexpr int L = D / 8;  // 16-byte chunks of a staged row
-      uint8_t* const to = static_cast<uint8_t*>(pieces ? static_cast<void*>(a.tile_part) : a.out);
       const bool store = !*abort_flag;
+      const int ch = r % L, shift = wide ? 2 : 1;
+      uint8_t* const to = (pieces ? reinterpret_cast<uint8_t*>(a.tile_part + piece0 * D) : static_cast<uint8_t*>(a.out) + (out0 << shift)) + 16 * ch;
+      const int64_t token_bytes = (int64_t)a.hq * D << shift;
       auto flush = [&](int pass) {
         tile_sync(1 + t);
 #pragma unroll 4
         for (int i = 0; i < L; i++) {
-          const int row = i * (TILE_M / L) + r / L, ch = r % L, rt = (int)((row * per16) >> 16), tk = work.tok0 + t * tpt + rt;
-          if (row < tpt * a.group && tk < work.sp.n && store) {
-            uint4 w;
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(stage + row * 2 * D + ((ch ^ (row & 7)) << 4)));
-            const int64_t at = (pieces ? piece0 + row : (work.sp.first + tk) * a.hq + work.head * a.group + row - rt * a.group) * D;
-            *reinterpret_cast<uint4*>(to + at * (wide ? 4 : 2) + pass * 2 * D + 16 * ch) = w;
-          }
+          const int row = i * (TILE_M / L) + r / L, at = row_at[t][row];
+          uint4 w;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(stage + row * 2 * D + ((ch ^ (row & 7)) << 4)));
+          uint8_t* const p = to + pass * 2 * D + (pieces ? (int64_t)(row * 4 * D) : (at & 255) * token_bytes + (((at >> 8) * D) << shift));
+          if (at >= 0 && store) *reinterpret_cast<uint4*>(p) = w;
         }
         tile_sync(1 + t);
       };
