@@ -13,6 +13,7 @@
 #include "device_utils.cuh"
 #include "handles.h"
 #include "kvcache.cuh"
+#include "tc_common.cuh"
 #include "turq_internal.h"
 
 namespace turq {
@@ -79,162 +80,237 @@ struct HeadRowsArgs {
   int* status;
 };
 
-// D / 8 lanes hold a row, eight elements each: a lane owns four pairs, so the rotation stays in its
-// registers. Pair p of the rotated part is (p, p + half_rot), or (2p, 2p + 1) interleaved; behind it
-// lane j simply has elements 8j .. 8j + 7. half_rot is a multiple of 4: no lane straddles the border.
-template <int D>
-__global__ void __launch_bounds__(256) head_rows_kernel(const HeadRowsArgs a) {
+// A block takes one token, D / 8 lanes a row (a head of q, k or v), ROUNDS rows of a token one behind the other with all their
+// loads in flight first: angles and weights are read once, and nothing is divided to find a row. A lane owns four pairs of a
+// row, so the rotation stays in its registers: pair p of the rotated part is (p, p + half_rot), or (2p, 2p + 1) interleaved;
+// behind it lane j simply has elements 8j .. 8j + 7. half_rot is a multiple of 4: no lane straddles the border.
+// X: the type of the rows; KIND: where keys go.
+enum RowKind { ROWS_DENSE, ROWS_16BIT, ROWS_Q8 };
+template <int D, int ROUNDS, int X, int KIND>
+__global__ void __launch_bounds__(256, ROUNDS == 1 ? 4 : 5) head_rows_kernel(const __grid_constant__ HeadRowsArgs a) {
   constexpr int L = D / 8;
-  const int j = threadIdx.x % L;
-  const int rows_per_token = a.hq + a.hkv * (a.cache.k ? 2 : 1);
-  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  // Lanes of rows that do not exist stay: the rows of a warp reduce together.
-  const bool live = row < a.n_tokens * rows_per_token;
-  const int64_t token = live ? row / rows_per_token : 0;
-  const int r = live ? (int)(row % rows_per_token) : 0;
-  const bool is_q = r < a.hq, is_v = r >= a.hq + a.hkv;
-  const int h = is_q ? r : is_v ? r - a.hq - a.hkv : r - a.hq;
-  const bool turn = a.table != nullptr && !is_v && 4 * j < a.half_rot;
-  const bool split = turn && !a.interleaved;       // this lane's pairs lie half_rot apart
-  const int e0 = split ? 4 * j : 8 * j, e1 = split ? a.half_rot + 4 * j : 8 * j + 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int j = threadIdx.x % L, groups = blockDim.x / L;
+  const int first = (int)blockIdx.y * ROUNDS * groups + (int)threadIdx.x / L;
+  const int rows = a.hq + a.hkv * (a.v ? 2 : 1);
+  const int64_t token = blockIdx.x;
+  const bool rot = a.table != nullptr && 4 * j < a.half_rot;  // this lane's pairs turn, where the row does
+  const bool split = rot && !a.interleaved;                   // and lie half_rot apart
 
-  float x[8];
-  const void* src = is_q ? a.q : is_v ? a.v : a.k;
-  const int64_t base = token * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) + (int64_t)h * D;
-  load4(src, a.x_dtype, base + e0, reinterpret_cast<float(&)[4]>(x[0]));
-  load4(src, a.x_dtype, base + e1, reinterpret_cast<float(&)[4]>(x[4]));
-  int64_t pos = 0;
+  // A row that does not exist (its lanes stay: the rows of a warp reduce together) reads the last one.
+  float x[ROUNDS][8];
+#pragma unroll
+  for (int u = 0; u < ROUNDS; u++) {
+    const int r = min(first + u * groups, rows - 1);
+    const bool is_q = r < a.hq, is_v = r >= a.hq + a.hkv, apart = split && !is_v;
+    const int64_t base = is_q ? token * a.q_stride + r * D : is_v ? token * a.v_stride + (r - a.hq - a.hkv) * D : token * a.k_stride + (r - a.hq) * D;
+    const void* src = is_q ? a.q : is_v ? a.v : a.k;
+    load4(src, X, base + (apart ? 4 * j : 8 * j), reinterpret_cast<float(&)[4]>(x[u][0]));
+    load4(src, X, base + (apart ? a.half_rot + 4 * j : 8 * j + 4), reinterpret_cast<float(&)[4]>(x[u][4]));
+  }
+  const int64_t slot = a.slots ? a.slots[token] : -1;
   bool known = true;
+  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
   if (a.table) {
-    pos = a.positions[token];
+    const int64_t pos = a.positions[token];
     known = pos >= 0 && pos < a.n_positions;
-    if (!known && live) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
-  }
-  const float* w = is_q ? a.wq : is_v ? nullptr : a.wk;
-  if (a.wq || a.wk) {  // the whole grid the same way: the shuffles need every lane
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; e++) ss += x[e] * x[e];
-#pragma unroll
-    for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-    if (w) {
-      const float rms = sqrtf(ss / D + a.eps);
-      float wv[8];
-      load4(w, TURQ_F32, e0, reinterpret_cast<float(&)[4]>(wv[0]));
-      load4(w, TURQ_F32, e1, reinterpret_cast<float(&)[4]>(wv[4]));
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = x[e] / rms * wv[e];
+    if (!known) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
+    if (rot && known) {
+      const float4* t = reinterpret_cast<const float4*>(a.table + pos * a.half_rot + 4 * j);
+      const float4 t0 = t[0], t1 = t[1];
+      c[0] = t0.x; c[1] = t0.z; c[2] = t1.x; c[3] = t1.z;
+      s[0] = t0.y; s[1] = t0.w; s[2] = t1.y; s[3] = t1.w;
     }
   }
-  if (turn && known) {
-    const float4* t = reinterpret_cast<const float4*>(a.table + pos * a.half_rot + 4 * j);
-    const float4 t0 = t[0], t1 = t[1];
-    const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float& p = split ? x[i] : x[2 * i];
-      float& q = split ? x[4 + i] : x[2 * i + 1];
-      const float px = p, qx = q;
-      p = px * c[i] - qx * s[i];
-      q = qx * c[i] + px * s[i];
-    }
-  }
-  if (!known) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = 0.f;
-  }
-
-  if (is_q || !a.cache.k) {
-    if (live) {
-      void* out = is_q ? a.q_out : a.k_out;
-      const int64_t o = (token * (is_q ? a.hq : a.hkv) + h) * D;
-      store4(out, a.out_dtype, o + e0, x);
-      store4(out, a.out_dtype, o + e1, x + 4);
-    }
-    if (!a.cache.k) return;
-  }
-  const int64_t slot = live && !is_q ? a.slots[token] : -1;
   const bool fits = slot < a.cache.n_pages * a.cache.page_size;
-  if (!fits) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
-  const bool write = live && !is_q && slot >= 0 && fits && known;
-  const int64_t at = write ? a.cache.row(slot, h) : 0;  // row of the planes
-  if (a.cache.dtype != TURQ_Q8_0) {
-    if (write) {
-      void* out = is_v ? a.cache.v : a.cache.k;
-      store4(out, a.cache.dtype, at * D + e0, x);
-      store4(out, a.cache.dtype, at * D + e1, x + 4);
-    }
-    return;
-  }
-  // Q8_0: lane j gets elements 8j .. 8j + 7, so that four lanes hold a block of 32. A group of four
-  // elements 4g .. 4g + 3 of a row whose pairs lie apart is the first half of lane g's registers, the second
-  // half of lane g - half_rot / 4's, or one of the two of lane g / 2.
-  if (a.table && !a.interleaved) {
-    float y[8];
+  if (KIND != ROWS_DENSE && !fits) *reinterpret_cast<volatile int*>(a.status) = TURQ_E_INVALID_ARG;
+  const bool write = KIND != ROWS_DENSE && slot >= 0 && fits && known;
+  const int64_t row0 = write ? a.cache.row(slot, 0) : 0;  // of the planes; a page's heads are page_size rows apart
+
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-      const int g = 2 * j + b, q4 = a.half_rot / 4;
-      const bool apart = a.table && !is_v;
-      const int from = apart && g < q4 ? g : apart && g < 2 * q4 ? g - q4 : g / 2;
-      const bool second = apart && g < q4 ? false : apart && g < 2 * q4 ? true : (g & 1) != 0;
+  for (int u = 0; u < ROUNDS; u++) {
+    const int r = first + u * groups;
+    const bool live = r < rows, is_q = r < a.hq, is_v = r >= a.hq + a.hkv;
+    float* const y = x[u];
+    if (a.wq || a.wk) {  // the whole grid the same way: the shuffles need every lane
+      float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float lo = __shfl_sync(0xFFFFFFFFu, x[i], from, L), hi = __shfl_sync(0xFFFFFFFFu, x[4 + i], from, L);
-        y[4 * b + i] = second ? hi : lo;
+      for (int e = 0; e < 8; e++) ss += y[e] * y[e];
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+      const float inv = 1.f / sqrtf(ss / D + a.eps);
+      const float* const w = is_q ? a.wq : is_v ? nullptr : a.wk;
+      if (w) {
+        float wv[8];
+        load4(w, TURQ_F32, split ? 4 * j : 8 * j, reinterpret_cast<float(&)[4]>(wv[0]));
+        load4(w, TURQ_F32, split ? a.half_rot + 4 * j : 8 * j + 4, reinterpret_cast<float(&)[4]>(wv[4]));
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = y[e] * inv * wv[e];
       }
     }
+    if (rot && !is_v) {
+      if (a.interleaved) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = y[e];
-  }
-  uint32_t w0, w1;
-  __half d;
-  quant_block_q8_0(x, w0, w1, d);
-  if (!write) return;
-  *reinterpret_cast<uint2*>((is_v ? a.cache.v : a.cache.k) + at * D + 8 * j) = make_uint2(w0, w1);
-  if ((j & 3) == 0) (is_v ? a.cache.vs : a.cache.ks)[at * (D / 32) + j / 4] = d;
-}
-
-// A group of D / 8 lanes per row of keys or values.
-template <int D>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvPages c, const int64_t* __restrict__ slots, int64_t n_tokens, int out_dtype,
-                                                      void* __restrict__ k_out, void* __restrict__ v_out, int* status) {
-  constexpr int L = D / 8;
-  const int j = threadIdx.x % L;
-  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (row >= 2 * n_tokens * c.n_heads) return;
-  const int64_t token = row / (2 * c.n_heads);
-  const int h = (int)(row % c.n_heads);
-  const bool is_v = row % (2 * c.n_heads) >= c.n_heads;
-  const int64_t slot = slots[token];
-  const bool fits = slot < c.n_pages * c.page_size;
-  if (!fits) *reinterpret_cast<volatile int*>(status) = TURQ_E_INVALID_ARG;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && fits) {
-    const int64_t at = c.row(slot, h);
-    const uint8_t* src = is_v ? c.v : c.k;
-    if (c.dtype == TURQ_Q8_0) {
-      const float d = __half2float((is_v ? c.vs : c.ks)[at * (D / 32) + j / 4]);
-      const uint2 t = *reinterpret_cast<const uint2*>(src + at * D + 8 * j);
+        for (int i = 0; i < 4; i++) {
+          const float p = y[2 * i], q = y[2 * i + 1];
+          y[2 * i] = p * c[i] - q * s[i];
+          y[2 * i + 1] = q * c[i] + p * s[i];
+        }
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = d * (float)(int8_t)((e < 4 ? t.x : t.y) >> (8 * (e & 3)));
-    } else {
-      load4(src, c.dtype, at * D + 8 * j, reinterpret_cast<float(&)[4]>(x[0]));
-      load4(src, c.dtype, at * D + 8 * j + 4, reinterpret_cast<float(&)[4]>(x[4]));
+        for (int i = 0; i < 4; i++) {
+          const float p = y[i], q = y[4 + i];
+          y[i] = p * c[i] - q * s[i];
+          y[4 + i] = q * c[i] + p * s[i];
+        }
+      }
+    }
+    if (!known) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = 0.f;
+    }
+    const int o0 = split && !is_v ? 4 * j : 8 * j, o1 = split && !is_v ? a.half_rot + 4 * j : 8 * j + 4;
+    if (live && (is_q || KIND == ROWS_DENSE)) {
+      void* out = is_q ? a.q_out : a.k_out;
+      const int64_t o = is_q ? (token * a.hq + r) * D : (token * a.hkv + r - a.hq) * D;
+      store4(out, a.out_dtype, o + o0, y);
+      store4(out, a.out_dtype, o + o1, y + 4);
+    }
+    if (KIND == ROWS_DENSE) continue;
+    const int h = is_v ? r - a.hq - a.hkv : r - a.hq;
+    const bool put = write && live && !is_q;
+    const int64_t at = row0 + (int64_t)(put ? h : 0) * a.cache.page_size;
+    if (KIND == ROWS_16BIT) {
+      if (put) {
+        void* out = is_v ? a.cache.v : a.cache.k;
+        store4(out, a.cache.dtype, at * D + o0, y);
+        store4(out, a.cache.dtype, at * D + o1, y + 4);
+      }
+      continue;
+    }
+    if (!__any_sync(0xFFFFFFFFu, put)) continue;
+    // Q8_0: lane j gets elements 8j .. 8j + 7, so that four lanes hold a block of 32. A group of four elements 4g .. 4g + 3 of a
+    // row whose pairs lie apart is the first half of lane g's registers, the second half of lane g - half_rot / 4's, or one
+    // of the two of lane g / 2.
+    if (a.table && !a.interleaved) {
+      float z[8];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const int g = 2 * j + b, q4 = a.half_rot / 4;
+        const int from = !is_v && g < q4 ? g : !is_v && g < 2 * q4 ? g - q4 : g / 2;
+        const bool second = !is_v && g < q4 ? false : !is_v && g < 2 * q4 ? true : (g & 1) != 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float lo = __shfl_sync(0xFFFFFFFFu, y[i], from, L), hi = __shfl_sync(0xFFFFFFFFu, y[4 + i], from, L);
+          z[4 * b + i] = second ? hi : lo;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = z[e];
+    }
+    uint32_t w0, w1;
+    __half d;
+    quant_block_q8_0(*reinterpret_cast<const float(*)[8]>(y), w0, w1, d);
+    if (put) {
+      *reinterpret_cast<uint2*>((is_v ? a.cache.v : a.cache.k) + at * D + 8 * j) = make_uint2(w0, w1);
+      if ((j & 3) == 0) (is_v ? a.cache.vs : a.cache.ks)[at * (D / 32) + j / 4] = d;
     }
   }
-  void* out = is_v ? v_out : k_out;
-  const int64_t o = (token * c.n_heads + h) * D + 8 * j;
-  store4(out, out_dtype, o, x);
-  store4(out, out_dtype, o + 4, x + 4);
 }
 
+// A block takes one token, D / 8 lanes a row of keys or values, ROUNDS of them one behind the other.
+template <int D, int ROUNDS>
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvPages c, const int64_t* __restrict__ slots, int out_dtype, void* __restrict__ k_out,
+                                                      void* __restrict__ v_out, int* status) {
+  constexpr int L = D / 8;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int j = threadIdx.x % L, groups = blockDim.x / L, first = (int)blockIdx.y * ROUNDS * groups + (int)threadIdx.x / L;
+  const int64_t token = blockIdx.x, slot = slots[token];
+  const bool fits = slot < c.n_pages * c.page_size, there = slot >= 0 && fits;
+  if (!fits) *reinterpret_cast<volatile int*>(status) = TURQ_E_INVALID_ARG;
+  const int64_t row0 = there ? c.row(slot, 0) : 0;
+  uint4 w[ROUNDS];
+  float d[ROUNDS];
+#pragma unroll
+  for (int u = 0; u < ROUNDS; u++) {
+    const int r = min(first + u * groups, 2 * c.n_heads - 1);
+    const bool is_v = r >= c.n_heads;
+    const int64_t at = row0 + (int64_t)(is_v ? r - c.n_heads : r) * c.page_size;
+    const uint8_t* src = is_v ? c.v : c.k;
+    if (c.dtype == TURQ_Q8_0) {
+      const uint2 t = *reinterpret_cast<const uint2*>(src + at * D + 8 * j);
+      w[u] = make_uint4(t.x, t.y, 0, 0);
+      d[u] = __half2float((is_v ? c.vs : c.ks)[at * (D / 32) + j / 4]);
+    } else {
+      w[u] = *reinterpret_cast<const uint4*>(src + (at * D + 8 * j) * 2);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < ROUNDS; u++) {
+    const int r = first + u * groups;
+    if (r >= 2 * c.n_heads) break;
+    const bool is_v = r >= c.n_heads;
+    const uint32_t t[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if (c.dtype == TURQ_Q8_0) {
+        x[e] = d[u] * (float)(int8_t)(t[e >> 2] >> (8 * (e & 3)));
+      } else {
+        const uint32_t bits = t[e >> 1] >> (16 * (e & 1));
+        x[e] = c.dtype == TURQ_BF16 ? __uint_as_float(bits << 16) : f16_bits_to_f32(bits);
+      }
+      if (!there) x[e] = 0.f;
+    }
+    const int64_t o = (token * c.n_heads + (is_v ? r - c.n_heads : r)) * D + 8 * j;
+    store4(is_v ? v_out : k_out, out_dtype, o, x);
+    store4(is_v ? v_out : k_out, out_dtype, o + 4, x + 4);
+  }
+}
+
+// Lanes for all rows of a token, 256 at most. Rounds: one where a call has so few tokens that blocks are what it lacks; otherwise two,
+// or four where a token has many wide rows (us, 1 / 2 / 4 rounds: 8192 tokens of 40 f32 rows of 128 64 / 69 / 53, 4099 of 16 bf16
+// rows of 128 11.8 / 11.0 / 12.8, 2049 of 60 bf16 rows of 64 11.0 / 10.4 / 11.3).
+struct RowGrid { dim3 grid, block; int rounds; };
+static RowGrid plan_rows(int64_t n_tokens, int rows, int head_dim, int most = 4) {
+  const int lanes = head_dim / 8;
+  RowGrid p;
+  p.rounds = n_tokens < 256 ? 1 : most == 4 && head_dim == 128 && rows >= 32 ? 4 : 2;
+  int threads = ((rows + p.rounds - 1) / p.rounds * lanes + 31) / 32 * 32;
+  if (threads > 256) threads = 256;
+  const int per_block = threads / lanes * p.rounds;
+  p.block = dim3(threads);
+  p.grid = dim3((unsigned)n_tokens, (unsigned)((rows + per_block - 1) / per_block));
+  return p;
+}
+
+template <int D, int X, int KIND>
+static cudaError_t launch_rows(const RowGrid& p, const HeadRowsArgs& a, cudaStream_t s) {
+  if (p.rounds == 1) return launch_pdl(head_rows_kernel<D, 1, X, KIND>, p.grid, p.block, 0, s, a);
+  if (D == 128 && p.rounds == 4) return launch_pdl(head_rows_kernel<D, D == 128 ? 4 : 2, X, KIND>, p.grid, p.block, 0, s, a);
+  return launch_pdl(head_rows_kernel<D, 2, X, KIND>, p.grid, p.block, 0, s, a);
+}
+template <int D, int X>
+static cudaError_t launch_rows_kind(const RowGrid& p, const HeadRowsArgs& a, cudaStream_t s) {
+  if (!a.cache.k) return launch_rows<D, X, ROWS_DENSE>(p, a, s);
+  return a.cache.dtype == TURQ_Q8_0 ? launch_rows<D, X, ROWS_Q8>(p, a, s) : launch_rows<D, X, ROWS_16BIT>(p, a, s);
+}
+template <int D>
+static cudaError_t launch_rows_type(const RowGrid& p, const HeadRowsArgs& a, cudaStream_t s) {
+  return a.x_dtype == TURQ_F32 ? launch_rows_kind<D, TURQ_F32>(p, a, s) : a.x_dtype == TURQ_BF16 ? launch_rows_kind<D, TURQ_BF16>(p, a, s) : launch_rows_kind<D, TURQ_F16>(p, a, s);
+}
 static cudaError_t launch_head_rows(int head_dim, const HeadRowsArgs& a, cudaStream_t s) {
-  const int64_t rows = a.n_tokens * (a.hq + a.hkv * (a.cache.k ? 2 : 1));
-  const int per_block = 256 / (head_dim / 8);
-  const unsigned grid = (unsigned)((rows + per_block - 1) / per_block);
-  if (head_dim == 64) head_rows_kernel<64><<<grid, 256, 0, s>>>(a);
-  else head_rows_kernel<128><<<grid, 256, 0, s>>>(a);
-  return cudaGetLastError();
+  const RowGrid p = plan_rows(a.n_tokens, a.hq + a.hkv * (a.v ? 2 : 1), head_dim);
+  return head_dim == 64 ? launch_rows_type<64>(p, a, s) : launch_rows_type<128>(p, a, s);
+}
+static cudaError_t launch_kv_read(int head_dim, const KvPages& pages, const int64_t* slots, int64_t n_tokens, int out_dtype, void* k_out, void* v_out, int* status,
+                                  cudaStream_t s) {
+  const RowGrid p = plan_rows(n_tokens, 2 * pages.n_heads, head_dim, 2);
+  auto go = [&](auto kernel) { return launch_pdl(kernel, p.grid, p.block, 0, s, pages, slots, out_dtype, k_out, v_out, status); };
+  if (head_dim == 64) return p.rounds == 1 ? go(kv_read_kernel<64, 1>) : go(kv_read_kernel<64, 2>);
+  return p.rounds == 1 ? go(kv_read_kernel<128, 1>) : go(kv_read_kernel<128, 2>);
 }
 
 }  // namespace turq
@@ -258,8 +334,7 @@ int32_t check_rows(turq_ctx* ctx, const void* p, int64_t stride, int64_t width, 
 int32_t check_tokens(turq_ctx* ctx, int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
   if (head_dim != 64 && head_dim != 128) return api_fail(ctx, TURQ_E_SHAPE, "head_dim must be 64 or 128");
   if (n_q_heads < 0 || n_kv_heads < 1 || n_q_heads > 65536 || n_kv_heads > 65536) return api_fail(ctx, TURQ_E_SHAPE, "head counts must be in 1..65536");
-  // one launch of 8 or 16 rows a block
-  if (n_tokens < 0 || n_tokens > INT32_MAX / 2 || n_tokens * ((int64_t)n_q_heads + 2 * (int64_t)n_kv_heads) > (int64_t)INT32_MAX * 8)
+  if (n_tokens < 0 || n_tokens > INT32_MAX / 2)
     return api_fail(ctx, TURQ_E_SHAPE, "n_tokens out of range");
   return TURQ_OK;
 }
@@ -546,12 +621,7 @@ int32_t turq_kv_read(turq_ctx* ctx, const turq_kv_cache* cache, const int64_t* d
   turq::DeviceScope on(ctx->device);
   if (on.status != cudaSuccess) return api_cuda_fail(ctx, on.status, "kv_read launch");
   const turq::KvPages pages = turq::pages_of(cache);
-  const int per_block = 256 / (d / 8);
-  const unsigned grid = (unsigned)((2 * n_tokens * hkv + per_block - 1) / per_block);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (d == 64) turq::kv_read_kernel<64><<<grid, 256, 0, s>>>(pages, dev_slots, n_tokens, out_dtype, dev_k_out, dev_v_out, ctx->dev_status);
-  else turq::kv_read_kernel<128><<<grid, 256, 0, s>>>(pages, dev_slots, n_tokens, out_dtype, dev_k_out, dev_v_out, ctx->dev_status);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = turq::launch_kv_read(d, pages, dev_slots, n_tokens, out_dtype, dev_k_out, dev_v_out, ctx->dev_status, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return api_cuda_fail(ctx, e, "kv_read launch");
   ctx->launches++;
   return TURQ_OK;
