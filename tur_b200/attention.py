@@ -177,7 +177,8 @@ class KvCache:
     def __init__(self, handle: ctypes.c_void_p, memory: torch.Tensor, dtype: GgmlDType, shape: tuple, ctx: _Context):
         self._h, self.memory, self.dtype, self._ctx, self._device = handle, memory, dtype, ctx, ctx.device
         lib = _lib.load()
-        self._append, self._attention, self._workspace = lib.turq_kv_append, lib.turq_kv_attention, lib.turq_kv_attention_workspace
+        self._append, self._write, self._read = lib.turq_kv_append, lib.turq_kv_write, lib.turq_kv_read
+        self._attention, self._workspace = lib.turq_kv_attention, lib.turq_kv_attention_workspace
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = shape
         self._scale = 1.0 / math.sqrt(self.head_dim)
         off = (ctypes.c_int64 * 4)()
@@ -232,34 +233,44 @@ class KvCache:
         dev, d = self._device, self.head_dim
         n, ks, vs = self._kv(k, v)
         nq, hq, qs = _rows(q, "q", dev, d)
-        if nq != n or q.dtype != k.dtype:
+        dtype = q.dtype
+        if nq != n or dtype is not k.dtype:
             raise TurqError(2, f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in tokens and type")
         if out_dtype not in _ROW_CODE:
             raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
-        wq, wk = _weights(table, d, dev, q_weight, k_weight)
+        if table._device != dev:
+            raise TurqError(1, f"the rotary table lives on {table.table.device}, the cache on cuda:{dev}")
+        wq = _vector(q_weight, "q_weight", dev, torch.float32, d) if q_weight is not None else None
+        wk = _vector(k_weight, "k_weight", dev, torch.float32, d) if k_weight is not None else None
         p_positions, p_slots = _vector(positions, "positions", dev, torch.int32, n), _vector(slots, "slots", dev, torch.int64, n)
-        qo = _out(q_out, "q_out", (n, hq, d), out_dtype, q)
-        st = self._append(self._ctx.handle, self._h, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[q.dtype], n, hq, wq, wk, eps,
-                          *table._args, p_positions, p_slots, _ROW_CODE[out_dtype], qo.data_ptr(), _stream_ptr(dev))
+        qo = q.new_empty((n, hq, d), dtype=out_dtype) if q_out is None else _out(q_out, "q_out", (n, hq, d), out_dtype, q)
+        t_ptr, t_n, t_dim, t_pairs = table._args
+        st = self._append(self._ctx.handle, self._h, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[dtype], n, hq, wq, wk, eps,
+                          t_ptr, t_n, t_dim, t_pairs, p_positions, p_slots, _ROW_CODE[out_dtype], qo.data_ptr(), _stream_ptr(dev))
         if st != 0:
             self._ctx.check(st)
         return qo
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Keys and values as they are into their slots, rounded to the cache's type or quantized."""
-        dev = self._ctx.device
+        dev = self._device
         n, ks, vs = self._kv(k, v)
-        self._ctx.check(_lib.load().turq_kv_write(self._ctx.handle, self._h, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[k.dtype], n,
-                                                  _vector(slots, "slots", dev, torch.int64, n), _stream_ptr(dev)))
+        st = self._write(self._ctx.handle, self._h, k.data_ptr(), ks, v.data_ptr(), vs, _ROW_CODE[k.dtype], n,
+                         _vector(slots, "slots", dev, torch.int64, n), _stream_ptr(dev))
+        if st != 0:
+            self._ctx.check(st)
 
     def read(self, slots: torch.Tensor, out_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values of the slots, [n, n_kv_heads, d] each; a negative slot reads as zeros."""
-        dev, n = self._ctx.device, slots.numel()
+        dev, n = self._device, slots.numel()
+        p_slots = _vector(slots, "slots", dev, torch.int64, None)
         if out_dtype not in _ROW_CODE:
             raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
-        k, v = (_out(None, "", (n, self.n_kv_heads, self.head_dim), out_dtype, self.memory) for _ in range(2))
-        self._ctx.check(_lib.load().turq_kv_read(self._ctx.handle, self._h, _vector(slots, "slots", dev, torch.int64, None), n,
-                                                 _ROW_CODE[out_dtype], k.data_ptr(), v.data_ptr(), _stream_ptr(dev)))
+        k = slots.new_empty((n, self.n_kv_heads, self.head_dim), dtype=out_dtype)
+        v = torch.empty_like(k)
+        st = self._read(self._ctx.handle, self._h, p_slots, n, _ROW_CODE[out_dtype], k.data_ptr(), v.data_ptr(), _stream_ptr(dev))
+        if st != 0:
+            self._ctx.check(st)
         return k, v
 
     def attend(self, q: torch.Tensor, starts: torch.Tensor, contexts: torch.Tensor, page_table: torch.Tensor, *, max_new: Optional[int] = None,
@@ -283,7 +294,12 @@ class KvCache:
         out_dtype = (out.dtype if out is not None else q.dtype) if out_dtype is None else out_dtype
         if out_dtype not in _ROW_CODE:
             raise TurqError(3, f"out_dtype {out_dtype} is none of float32, float16, bfloat16")
-        y = _out(out, "out", (n, hq, d), out_dtype, q)
+        if out is not None:
+            y = _out(out, "out", (n, hq, d), out_dtype, q)
+        elif out_dtype is q.dtype and q.dim() == 3 and q.is_contiguous():
+            y = torch.empty_like(q)
+        else:
+            y = q.new_empty((n, hq, d), dtype=out_dtype)
         nbytes = self._workspace(self._h, n, n_seqs, hq, max_new, max_context)
         ws = y.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         st = self._attention(self._ctx.handle, self._h, q.data_ptr(), qs, _ROW_CODE[q.dtype], n, hq, p_starts, p_contexts, p_table, pages, n_seqs,
