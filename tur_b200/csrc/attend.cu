@@ -27,11 +27,11 @@ static AttendWorkspace attend_workspace(const turq_kv_cache* kc, int64_t n_token
   w.tokens = group <= TOKEN_ROWS;
   w.tiles = most * group > TOKEN_ROWS;
   if (w.tokens) {
-    const TokenPlan p = plan_tokens((int64_t)n_seqs * kc->n_kv_heads, max_context, kc->sm_count);
+    w.part_rows = (int)(w.tiles ? TOKEN_ROWS : most * group);
+    const TokenPlan p = plan_tokens((int64_t)n_seqs * kc->n_kv_heads, max_context, kc->sm_count, token_ctas(kc->dtype == TURQ_Q8_0, w.part_rows <= 8));
     w.chunk = (int)p.chunk;
     w.max_chunks = (int)p.chunks;
     w.cluster = p.cluster;
-    w.part_rows = (int)(w.tiles ? TOKEN_ROWS : most * group);
     if (p.chunks > 1 && !p.cluster) {
       const size_t rows = (size_t)n_seqs * kc->n_kv_heads * p.chunks * w.part_rows;
       w.off_ml = up(rows * kc->head_dim * 4);

@@ -36,18 +36,20 @@ TQ_HD int64_t keys_seen(const Span& s, int64_t t, bool causal) {
 
 // ---- single tokens: up to TOKEN_ROWS rows (new tokens x query heads of a key head)
 constexpr int TOKEN_ROWS = 16;
-// The contexts of a call are cut into chunks of one length, a CTA each, three CTAs at a time on an SM. A CTA has
+// The contexts of a call are cut into chunks of one length, a CTA each, three or four CTAs at a time on an SM. A CTA has
 // costs of its own (the way from the lengths over the page table to the first keys, the join of its warps) worth
-// TOKEN_OVERHEAD keys, and the last wave is as long as a full one, so the length is the one whose waves x (keys +
-// overhead) is least. Measured, us a call (bf16 24 x 4096, Q8_0 24 x 4096, f16 2 x 120000 keys; 8 heads of 128): 256 keys
-// 81, 92, -; 512 keys 76, 76, 176; 1024 keys 70, 69, 189; the rule's own 70, 69, 173.
-constexpr int TOKEN_STEP = 128, TOKEN_CHUNK_MAX = 8192, TOKEN_OVERHEAD = 96, TOKEN_CTAS = 3;
-inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64_t max_context, int sms) {
+// TOKEN_OVERHEAD keys, and 1 to 4 CTAs at a time on an SM take TOKEN_DEPTH times as long as the keys of one of them would if they did
+// not share it; a wave that is not the only one costs a full one. The length with the least cost is taken. Measured, us (8 heads of 128): one user at 16384 keys in bf16 in chunks of 256 18.4, 512 13.1, 1024 17.3; 24 users at 4096
+// 256 81, 1024 70, 2048 70; two at 120000 1024 156, 4480 148.
+constexpr int TOKEN_STEP = 128, TOKEN_CHUNK_MAX = 8192, TOKEN_OVERHEAD = 96;
+constexpr int TOKEN_DEPTH[5] = {0, 140, 162, 216, 264};  // hundredths
+constexpr int token_ctas(bool q8, bool eight_rows) { return q8 && eight_rows ? 4 : 3; }
+inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64_t max_context, int sms, int ctas) {
   int64_t best = TOKEN_STEP, cost = -1;
   for (int64_t c = TOKEN_STEP; c <= TOKEN_CHUNK_MAX; c += TOKEN_STEP) {
-    const int64_t chunks = max_context <= c ? 1 : (max_context + c - 1) / c, slots = (int64_t)TOKEN_CTAS * sms;
-    const int64_t keys = c < max_context ? c : max_context;
-    const int64_t t = (pairs * chunks + slots - 1) / slots * (keys + TOKEN_OVERHEAD);
+    const int64_t chunks = max_context <= c ? 1 : (max_context + c - 1) / c, n = pairs * chunks, slots = (int64_t)ctas * sms;
+    const int64_t keys = c < max_context ? c : max_context, deep = (n + sms - 1) / sms;
+    const int64_t t = (n > slots ? (n + slots - 1) / slots * TOKEN_DEPTH[ctas] : TOKEN_DEPTH[deep]) * (keys + TOKEN_OVERHEAD);
     if (cost < 0 || t < cost) {
       cost = t;
       best = c;
@@ -64,13 +66,13 @@ inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64
 // the host 5); 8192 keys in chunks of 512 12.3 against 9.9, which is why a chunk may not be longer than 256 for it.
 constexpr int TOKEN_CLUSTER = 16, TOKEN_CLUSTER_KEYS = 256;
 struct TokenPlan { int64_t chunk, chunks; bool cluster; };
-inline TokenPlan plan_tokens(int64_t pairs, int64_t max_context, int sms) {
+inline TokenPlan plan_tokens(int64_t pairs, int64_t max_context, int sms, int ctas) {
   TokenPlan p;
   const int64_t sixteenth = (max_context + TOKEN_CLUSTER * TOKEN_STEP - 1) / (TOKEN_CLUSTER * TOKEN_STEP) * TOKEN_STEP;
-  p.chunk = plan_token_chunk(pairs, max_context, sms);
+  p.chunk = plan_token_chunk(pairs, max_context, sms, ctas);
   if (sixteenth > p.chunk && sixteenth <= TOKEN_CLUSTER_KEYS && pairs * TOKEN_CLUSTER <= sms) p.chunk = sixteenth;
   p.chunks = max_context <= p.chunk ? 1 : (max_context + p.chunk - 1) / p.chunk;
-  p.cluster = p.chunks > 1 && p.chunks <= TOKEN_CLUSTER && pairs * p.chunks <= (int64_t)(p.chunks <= 8 ? TOKEN_CTAS : 1) * sms;
+  p.cluster = p.chunks > 1 && p.chunks <= TOKEN_CLUSTER && pairs * p.chunks <= (int64_t)(p.chunks <= 8 ? ctas : 1) * sms;
   return p;
 }
 

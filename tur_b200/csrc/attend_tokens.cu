@@ -23,19 +23,23 @@
 namespace turq {
 
 constexpr int TOK_WARPS = 4;
-constexpr int TOK_STAGES = 2;
 
-// The bytes of a step: 8 KB of keys and values, with the scales of Q8_0 behind them.
-template <int D, bool Q8> struct TokGeom {
+// A warp's ring: steps of 8 KB of keys and values; of 4 KB for Q8_0 where at most eight query rows leave registers for a fourth
+// CTA an SM (their conversion waits for itself: 24 users at 4096 keys 66 us with three, 58 with four, two at 120000 123 and 97). Scales of
+// Q8_0 lie behind the steps.
+template <int D, bool Q8, int NR> struct TokGeom {
+  static constexpr bool FOUR = Q8 && NR == 1;
+  static constexpr int CTAS = token_ctas(Q8, NR == 1);
+  static constexpr int STAGES = FOUR && D == 128 ? 3 : 2;
+  static constexpr int HALF = FOUR ? 2048 : 4096;      // bytes of the keys of a step, and of its values
   static constexpr int ROW = Q8 ? D : 2 * D;           // bytes of a key
-  static constexpr int KEYS = 4096 / ROW;              // 16 to 64
+  static constexpr int KEYS = HALF / ROW;              // 16 to 64
   static constexpr int BOX = 16 * (Q8 ? D : 128);      // one copy: 16 keys of a 128-byte column block, or of int8
   static constexpr int SC = Q8 ? 16 * (D / 32) * 2 : 0;  // scales of 16 keys: 128 or 64 bytes,
   static constexpr int SC_AT = Q8 ? 128 : 0;             // each copy to a 128-byte boundary, as tensor copies ask for
-  static constexpr int STAGE = 8192 + (Q8 ? 1024 : 0);
-  static constexpr int RING = TOK_STAGES * STAGE;
+  static constexpr int SCALES = KEYS / 16 * 2 * SC_AT;   // of a step
+  static constexpr int RING = (STAGES * (2 * HALF + SCALES) + 1023) / 1024 * 1024;
   static constexpr int RES = D + 4;                    // floats from one result row to the next: four row pairs x eight columns meet all banks
-  static_assert(KEYS / 16 * 2 * SC_AT <= 1024 && SC <= 128, "scales of a step");
   static_assert(RING >= 16 * RES * 4 + 128, "the ring holds a warp's result");
 };
 
@@ -83,9 +87,9 @@ __device__ __forceinline__ void copy_box2(uint32_t dst, const CUtensorMap* map, 
 struct TokMaps { CUtensorMap k, v, ks, vs; };
 
 template <int D, bool Q8, bool BF, int NR /* tiles of 8 query rows */>
-__global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kernel(const __grid_constant__ TokMaps maps, const __grid_constant__ AttendArgs a) {
-  using G = TokGeom<D, Q8>;
-  constexpr int KEYS = G::KEYS, KT = KEYS / 16, KS = D / 16, MT = D / 16, HALVES = Q8 ? 1 : D / 64;
+__global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) attend_tokens_kernel(const __grid_constant__ TokMaps maps, const __grid_constant__ AttendArgs a) {
+  using G = TokGeom<D, Q8, NR>;
+  constexpr int TOK_STAGES = G::STAGES, KEYS = G::KEYS, KT = KEYS / 16, KS = D / 16, MT = D / 16, HALVES = Q8 ? 1 : D / 64;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) uint64_t full[TOK_WARPS][TOK_STAGES];
   __shared__ int pages[TOKEN_CHUNK_MAX / 16];
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
   // one step's copies: only boxes that begin inside the context; a page that the cache does not have reads as zeros
   auto issue = [&](int step, int stage) {
     const int k0 = step * KEYS, boxes = min(KT, (keys - k0 + 15) / 16);
-    const uint32_t bar = s_u32(&full[warp][stage]), at = ring + stage * G::STAGE;
+    const uint32_t bar = s_u32(&full[warp][stage]), at = ring + stage * 2 * G::HALF, sc = ring + TOK_STAGES * 2 * G::HALF + stage * G::SCALES;
     bar_expect_tx(&full[warp][stage], boxes * (2 * HALVES * G::BOX + 2 * G::SC));
 #pragma unroll
     for (int b = 0; b < KT; b++) {
@@ -139,11 +143,11 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
 #pragma unroll
       for (int h = 0; h < HALVES; h++) {
         copy_box3(at + (b * HALVES + h) * G::BOX, &maps.k, 64 * h, y, z, bar);
-        copy_box3(at + 4096 + (b * HALVES + h) * G::BOX, &maps.v, 64 * h, y, z, bar);
+        copy_box3(at + G::HALF + (b * HALVES + h) * G::BOX, &maps.v, 64 * h, y, z, bar);
       }
       if (Q8) {
-        copy_box2(at + 8192 + b * G::SC_AT, &maps.ks, y * (D / 32), z, bar);
-        copy_box2(at + 8192 + (KT + b) * G::SC_AT, &maps.vs, y * (D / 32), z, bar);
+        copy_box2(sc + b * G::SC_AT, &maps.ks, y * (D / 32), z, bar);
+        copy_box2(sc + (KT + b) * G::SC_AT, &maps.vs, y * (D / 32), z, bar);
       }
     }
   };
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
       report(a.status, TURQ_E_TIMEOUT);
     }
     __syncwarp();
-    const uint32_t at = ring + stage * G::STAGE;
+    const uint32_t at = ring + stage * 2 * G::HALF, sc = ring + TOK_STAGES * 2 * G::HALF + stage * G::SCALES;
     const int k0 = step * KEYS;
 
     // S^T: lane (g, c) gets keys g and g + 8 of a tile for rows 2c, 2c + 1
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
           for (int j = 0; j < NR; j++) mma_16816<BF>(s[kt][j], k, qf[j][i][0], qf[j][i][1]);
         }
       } else {
-        const uint32_t kb = at + kt * G::BOX + g * D, sb = at + 8192 + kt * G::SC_AT + (g * (D / 32) + c * D / 128) * 2;
+        const uint32_t kb = at + kt * G::BOX + g * D, sb = sc + kt * G::SC_AT + (g * (D / 32) + c * D / 128) * 2;
         uint16_t s0, s1;
         asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s0) : "r"(sb));
         asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s1) : "r"(sb + 8 * (D / 32) * 2));
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
     for (int kt = 0; kt < KT; kt++) {
       const int live = keys - k0 - 16 * kt;  // keys of this box that exist: what lies behind may be anything, and 0 x NaN is NaN
       if (!Q8) {
-        const uint32_t vb = at + 4096 + kt * HALVES * G::BOX;
+        const uint32_t vb = at + G::HALF + kt * HALVES * G::BOX;
         if (live < 16) {
           for (int i = lane; i < 16 * D / 8; i += 32) {
             const int row = i & 15, ch = i >> 4;
@@ -333,10 +337,10 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
       } else {
         // Lane (g, c): D / 8 columns from D/8 g of keys 2c, 2c + 1, 2c + 8, 2c + 9; tile i's rows g and g + 8 are its columns 2i and
         // 2i + 1. Behind the context's end the quants are some bytes, and a scale of zero makes them zeros.
-        const uint32_t vb = at + 4096 + kt * G::BOX, sb = at + 8192 + (KT + kt) * G::SC_AT + (g * D / 256) * 2;
+        const uint32_t vb = at + G::HALF + kt * G::BOX, sb = sc + (KT + kt) * G::SC_AT + (g * D / 256) * 2;
         constexpr int W = D / 32;  // words of a key
         uint32_t w[4][W];
-        uint16_t sc[4];
+        uint16_t vs[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const int row = 2 * c + (i & 1) + 8 * (i >> 1);
@@ -346,10 +350,10 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TOKEN_CTAS) attend_tokens_kern
           else
             asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[i][0]), "=r"(w[i][1])
                          : "r"(vb + row * D + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + (g & 1) * 8));
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc[i]) : "r"(sb + row * (D / 32) * 2));
-          if (row >= live) sc[i] = 0;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(vs[i]) : "r"(sb + row * (D / 32) * 2));
+          if (row >= live) vs[i] = 0;
         }
-        const __half2 sc01 = __halves2half2(__ushort_as_half(sc[0]), __ushort_as_half(sc[1])), sc23 = __halves2half2(__ushort_as_half(sc[2]), __ushort_as_half(sc[3]));
+        const __half2 sc01 = __halves2half2(__ushort_as_half(vs[0]), __ushort_as_half(vs[1])), sc23 = __halves2half2(__ushort_as_half(vs[2]), __ushort_as_half(vs[3]));
         const __half2 off = __float2half2_rn(1152.f);
 #pragma unroll
         for (int i = 0; i < W; i++) {
@@ -522,7 +526,7 @@ __global__ void __launch_bounds__(256) join_tokens_kernel(const __grid_constant_
 
 template <int D, bool Q8, bool BF, int NR>
 static cudaError_t launch_tokens_rows(const turq_kv_cache* kc, const AttendArgs& a, cudaStream_t s, int* launches) {
-  using G = TokGeom<D, Q8>;
+  using G = TokGeom<D, Q8, NR>;
   constexpr int SMEM = TOK_WARPS * G::RING + 1024;
   static PerDeviceOnce configured;
   int dev = 0;
