@@ -259,10 +259,6 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
   volatile int* const abort_flag = &abort_word;
   const int tpt = TILE_M / a.group;  // tokens of a tile
 
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&tmem_slot)), "n"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
   if (threadIdx.x == 32) {
     for (int i = 0; i < 2; i++) { bar_init(&q_full[i], 4); bar_init(&s_full[i], 1); bar_init(&p_full[i][0], 4); bar_init(&p_full[i][1], 4); bar_init(&s_read[i], 4); bar_init(&o_full[i], 1); }
     for (int i = 0; i < ST; i++) { bar_init(&kv_full[i], Q8 ? 4 : 1); bar_init(&kv_empty[i], 1); }
@@ -279,14 +275,16 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 0) find_work(a, 2 * tpt, &work, lane);
+  __syncthreads();
+  if (!work.live) return;  // (before anything is allocated: a call has blocks for the most tiles and pieces that there may be)
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(&tmem_slot)), "n"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = tmem_slot;
-  if (!work.live) {
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
-    return;
-  }
   const Span sp = work.sp;
   const int seq = work.seq, head = work.head, begin = work.begin, n_iter = work.end - work.begin;
   const int tiles = sp.n - work.tok0 > tpt ? 2 : 1;  // row tiles with rows
