@@ -268,9 +268,10 @@ int32_t turq_lm_head_topk(turq_ctx* ctx, const turq_qtensor* qt, const void* dev
  * src/models/granite_41.rs: the same without head norms; src/models/kv_cache.rs:288-525: pages).
  * Head dimensions are 64 or 128. Rows of q, k and v are tokens: [n_tokens, heads * head_dim] with
  * heads side by side, `*_stride` elements from one token to the next (attn_q|k|v as views of one
- * matrix are fine). Bases are 16-byte aligned and strides are whole multiples of 16 bytes. None of
- * these calls allocates, synchronizes or uses memory of the context beyond its status word, so
- * calls on different streams and replays of captured graphs do not meet in it. */
+ * matrix are fine). Bases are 16-byte aligned and strides are whole multiples of 16 bytes. But for
+ * turq_kv_cache_create without memory, none of these calls allocates, synchronizes or uses memory of
+ * the context beyond its status word, so calls on different streams and replays of captured
+ * graphs do not meet in it; the caller's current device stays what it is. */
 
 /* cos and sin of position * host_freqs[i] times `scale`, computed in 64 bits: dev_table is f32
  * [n_positions, n_freqs, 2], 16-byte aligned. n_freqs (half the rotated part of a head) is a

@@ -16,6 +16,10 @@
 //   ln -> projections (src/models/qwen3.rs:633-638)          turq::rmsnorm_forward_multi
 //   lm_head -> LogitsProcessor::sample                       turq::QMatMul::lm_head_topk
 //     (src/backend/engine.rs:528-529, 810-824)
+//   RoPE tables (src/models/qwen3.rs:64-78)                  turq::Rotary, rope_table
+//   q/k norm, RoPE (src/models/qwen3.rs:277-290)             turq::qk_norm_rope
+//   PagedKvCache (src/models/kv_cache.rs:288-525), attention turq::KvCache::{append, write, read, attend}
+//     (src/models/qwen3.rs:290-505)
 //
 // Header-only; link with libturq.so. Device pointers are the caller's (any allocator).
 #pragma once
@@ -195,6 +199,84 @@ inline void rmsnorm_forward_multi(const std::vector<const QMatMul*>& mms, const 
   c->check(turq_rmsnorm_qmatmul_multi(c->handle(), static_cast<int32_t>(qts.size()), qts.data(), dev_x, static_cast<int32_t>(x_dtype), m,
                                       dev_norm_weight, eps, dev_h_out, dev_ys.data(), static_cast<int32_t>(mode), nullptr, stream));
 }
+
+// A table of cos and sin in device memory ([n_positions, rotary_dim / 2, 2] f32) and how it is read.
+struct Rotary {
+  const float* dev_table = nullptr;
+  int64_t n_positions = 0;
+  int32_t rotary_dim = 0;
+  bool interleaved = false;
+};
+inline void rope_table(const Context& ctx, const std::vector<double>& freqs, int64_t n_positions, float* dev_table, double scale = 1.0,
+                       void* stream = nullptr) {
+  ctx.check(turq_rope_table(ctx.handle(), freqs.data(), static_cast<int32_t>(freqs.size()), n_positions, scale, dev_table, stream));
+}
+
+// Rows of heads in device memory: [n, heads * head_dim], `stride` elements from one token to the next.
+struct HeadRows {
+  const void* dev = nullptr;
+  int64_t stride = 0;
+};
+
+// RMSNorm of every head (where a weight is given) and rotation of q and k into dense tensors of out_dtype.
+inline void qk_norm_rope(const Context& ctx, HeadRows q, HeadRows k, GgmlDType x_dtype, int64_t n, int32_t n_heads, int32_t n_kv_heads,
+                         int32_t head_dim, const float* dev_q_weight, const float* dev_k_weight, float eps, const Rotary& rotary,
+                         const int32_t* dev_positions, GgmlDType out_dtype, void* dev_q_out, void* dev_k_out, void* stream = nullptr) {
+  ctx.check(turq_qk_norm_rope(ctx.handle(), q.dev, q.stride, k.dev, k.stride, static_cast<int32_t>(x_dtype), n, n_heads, n_kv_heads, head_dim,
+                              dev_q_weight, dev_k_weight, eps, rotary.dev_table, rotary.n_positions, rotary.rotary_dim, rotary.interleaved,
+                              dev_positions, static_cast<int32_t>(out_dtype), dev_q_out, dev_k_out, stream));
+}
+
+// One layer's keys and values in pages (F16, BF16 or Q8_0). dev_memory: the caller's, turq_kv_cache_bytes of it, or null.
+class KvCache {
+ public:
+  KvCache(std::shared_ptr<Context> ctx, GgmlDType dtype, int64_t n_pages, int32_t page_size, int32_t n_kv_heads, int32_t head_dim,
+          void* dev_memory = nullptr, size_t nbytes = 0)
+      : ctx_(std::move(ctx)) {
+    ctx_->check(turq_kv_cache_create(ctx_->handle(), static_cast<int32_t>(dtype), n_pages, page_size, n_kv_heads, head_dim, dev_memory, nbytes, &h_));
+  }
+  ~KvCache() {
+    if (h_) turq_kv_cache_free(h_);
+  }
+  KvCache(const KvCache&) = delete;
+  KvCache& operator=(const KvCache&) = delete;
+
+  // Norms and rotation of q and k, k and v into their slots, q into a dense tensor: one pass.
+  void append(HeadRows q, HeadRows k, HeadRows v, GgmlDType x_dtype, int64_t n, int32_t n_heads, const float* dev_q_weight,
+              const float* dev_k_weight, float eps, const Rotary& rotary, const int32_t* dev_positions, const int64_t* dev_slots,
+              GgmlDType out_dtype, void* dev_q_out, void* stream = nullptr) {
+    ctx_->check(turq_kv_append(ctx_->handle(), h_, q.dev, q.stride, k.dev, k.stride, v.dev, v.stride, static_cast<int32_t>(x_dtype), n, n_heads,
+                               dev_q_weight, dev_k_weight, eps, rotary.dev_table, rotary.n_positions, rotary.rotary_dim, rotary.interleaved,
+                               dev_positions, dev_slots, static_cast<int32_t>(out_dtype), dev_q_out, stream));
+  }
+  void write(HeadRows k, HeadRows v, GgmlDType x_dtype, int64_t n, const int64_t* dev_slots, void* stream = nullptr) {
+    ctx_->check(turq_kv_write(ctx_->handle(), h_, k.dev, k.stride, v.dev, v.stride, static_cast<int32_t>(x_dtype), n, dev_slots, stream));
+  }
+  void read(const int64_t* dev_slots, int64_t n, GgmlDType out_dtype, void* dev_k, void* dev_v, void* stream = nullptr) const {
+    ctx_->check(turq_kv_read(ctx_->handle(), h_, dev_slots, n, static_cast<int32_t>(out_dtype), dev_k, dev_v, stream));
+  }
+  // The new tokens of n_seqs sequences over their pages; arrays as turq_kv_attention describes them.
+  struct Batch {
+    const int32_t *dev_starts = nullptr, *dev_contexts = nullptr, *dev_page_table = nullptr;
+    int64_t table_stride = 0;
+    int32_t n_seqs = 0;
+    int64_t n_tokens = 0, max_new = 0, max_context = 0;
+  };
+  size_t workspace(const Batch& b, int32_t n_heads) const {
+    return turq_kv_attention_workspace(h_, b.n_tokens, b.n_seqs, n_heads, b.max_new, b.max_context);
+  }
+  void attend(HeadRows q, GgmlDType q_dtype, int32_t n_heads, const Batch& b, float scale, bool causal, GgmlDType out_dtype, void* dev_out,
+              void* dev_workspace, size_t workspace_bytes, void* stream = nullptr) const {
+    ctx_->check(turq_kv_attention(ctx_->handle(), h_, q.dev, q.stride, static_cast<int32_t>(q_dtype), b.n_tokens, n_heads, b.dev_starts, b.dev_contexts,
+                                  b.dev_page_table, b.table_stride, b.n_seqs, b.max_new, b.max_context, scale, causal, static_cast<int32_t>(out_dtype),
+                                  dev_out, dev_workspace, workspace_bytes, stream));
+  }
+  turq_kv_cache* handle() const { return h_; }
+
+ private:
+  std::shared_ptr<Context> ctx_;
+  turq_kv_cache* h_ = nullptr;
+};
 
 // The `Quantized` arm of tur's LinearX: QMatMul plus an optional f32 bias in device memory
 // (the add is fused into the matmul epilogue).

@@ -438,6 +438,187 @@ impl QMatMul {
     }
 }
 
+/// Rows of heads in device memory: `[n, heads * head_dim]`, `stride` elements from one token to the next.
+#[derive(Debug, Clone, Copy)]
+pub struct HeadRows {
+    pub dev: *const c_void,
+    pub stride: i64,
+}
+
+/// A table of cos and sin (`turq_rope_table`; `src/models/qwen3.rs:64-78`) and how it is read.
+#[derive(Debug, Clone, Copy)]
+pub struct Rotary {
+    pub dev_table: *const f32,
+    pub n_positions: i64,
+    pub rotary_dim: i32,
+    pub interleaved: bool,
+}
+
+/// The new tokens of several sequences over their pages (`turq_kv_attention`).
+#[derive(Debug, Clone, Copy)]
+pub struct Batch {
+    pub dev_starts: *const i32,
+    pub dev_contexts: *const i32,
+    pub dev_page_table: *const i32,
+    pub table_stride: i64,
+    pub n_seqs: i32,
+    pub n_tokens: i64,
+    pub max_new: i64,
+    pub max_context: i64,
+}
+
+/// One layer's keys and values in pages (`PagedKvCache`, `src/models/kv_cache.rs:288-525`).
+pub struct KvCache {
+    ctx: Arc<Context>,
+    h: *mut sys::turq_kv_cache,
+}
+
+// SAFETY: the handle's host state does not change after its creation; calls on one cache are ordered by their streams.
+unsafe impl Send for KvCache {}
+
+impl KvCache {
+    /// Pages of `page_size` tokens in F16, BF16 or Q8_0, allocated and zeroed by the library.
+    pub fn new(ctx: &Arc<Context>, dtype: GgmlDType, n_pages: usize, page_size: usize, n_kv_heads: usize, head_dim: usize) -> Result<Self> {
+        let mut h: *mut sys::turq_kv_cache = ptr::null_mut();
+        // SAFETY: live context, valid out pointer.
+        let st = unsafe {
+            sys::turq_kv_cache_create(
+                ctx.h,
+                dtype as i32,
+                n_pages as i64,
+                page_size as i32,
+                n_kv_heads as i32,
+                head_dim as i32,
+                ptr::null_mut(),
+                0,
+                &mut h,
+            )
+        };
+        ctx.check(st)?;
+        Ok(Self { ctx: Arc::clone(ctx), h })
+    }
+
+    /// Norms and rotation of q and k (`src/models/qwen3.rs:277-290`), k and v into their slots, q into a dense tensor.
+    ///
+    /// # Safety
+    /// The pointers must be device pointers on the cache's device with the sizes `turq_kv_append` states, and stay valid until the
+    /// stream has run the work.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn append(
+        &self,
+        q: HeadRows,
+        k: HeadRows,
+        v: HeadRows,
+        x_dtype: GgmlDType,
+        n: usize,
+        n_heads: usize,
+        dev_q_weight: *const f32,
+        dev_k_weight: *const f32,
+        eps: f32,
+        rotary: &Rotary,
+        dev_positions: *const i32,
+        dev_slots: *const i64,
+        out_dtype: GgmlDType,
+        dev_q_out: *mut c_void,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        // SAFETY: forwarded contract of this function.
+        let st = unsafe {
+            sys::turq_kv_append(
+                self.ctx.h,
+                self.h,
+                q.dev,
+                q.stride,
+                k.dev,
+                k.stride,
+                v.dev,
+                v.stride,
+                x_dtype as i32,
+                n as i64,
+                n_heads as i32,
+                dev_q_weight,
+                dev_k_weight,
+                eps,
+                rotary.dev_table,
+                rotary.n_positions,
+                rotary.rotary_dim,
+                i32::from(rotary.interleaved),
+                dev_positions,
+                dev_slots,
+                out_dtype as i32,
+                dev_q_out,
+                stream,
+            )
+        };
+        self.ctx.check(st)
+    }
+
+    /// Bytes of workspace that `attend` needs for these bounds.
+    pub fn workspace(&self, b: &Batch, n_heads: usize) -> usize {
+        // SAFETY: live handle.
+        unsafe { sys::turq_kv_attention_workspace(self.h, b.n_tokens, b.n_seqs, n_heads as i32, b.max_new, b.max_context) }
+    }
+
+    /// softmax(scale q K^T) V of the new tokens over their pages (`src/models/qwen3.rs:290-505`).
+    ///
+    /// # Safety
+    /// As for `append`, with the sizes `turq_kv_attention` states.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn attend(
+        &self,
+        q: HeadRows,
+        q_dtype: GgmlDType,
+        n_heads: usize,
+        b: &Batch,
+        scale: f32,
+        causal: bool,
+        out_dtype: GgmlDType,
+        dev_out: *mut c_void,
+        dev_workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> Result<()> {
+        // SAFETY: forwarded contract of this function.
+        let st = unsafe {
+            sys::turq_kv_attention(
+                self.ctx.h,
+                self.h,
+                q.dev,
+                q.stride,
+                q_dtype as i32,
+                b.n_tokens,
+                n_heads as i32,
+                b.dev_starts,
+                b.dev_contexts,
+                b.dev_page_table,
+                b.table_stride,
+                b.n_seqs,
+                b.max_new,
+                b.max_context,
+                scale,
+                i32::from(causal),
+                out_dtype as i32,
+                dev_out,
+                dev_workspace,
+                workspace_bytes,
+                stream,
+            )
+        };
+        self.ctx.check(st)
+    }
+}
+
+impl Drop for KvCache {
+    fn drop(&mut self) {
+        if !self.h.is_null() {
+            // SAFETY: the handle came from the library and is released exactly once.
+            unsafe {
+                sys::turq_kv_cache_free(self.h);
+            }
+        }
+    }
+}
+
 /// tur's quantized linear (`LinearX::Quantized { qmatmul, bias }`, `linear.rs:13-16`).
 #[derive(Clone)]
 pub struct LinearX {
