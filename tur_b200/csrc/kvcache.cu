@@ -46,6 +46,11 @@ __device__ __forceinline__ void load4(const void* p, int dtype, int64_t i, float
   }
   v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
 }
+// 1 / sqrt(v): the hardware's estimate (2^-22) and one step of Newton's method.
+__device__ __forceinline__ float inverse_root(float v) {
+  const float r = rsqrtf(v);
+  return r * fmaf(-0.5f * v * r, r, 1.5f);
+}
 __device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const float* v) {
   if (dtype == TURQ_F32) {
     *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
@@ -87,7 +92,7 @@ struct HeadRowsArgs {
 // X: the type of the rows; KIND: where keys go.
 enum RowKind { ROWS_DENSE, ROWS_16BIT, ROWS_Q8 };
 template <int D, int ROUNDS, int X, int KIND>
-__global__ void __launch_bounds__(256, ROUNDS == 1 ? 4 : 5) head_rows_kernel(const __grid_constant__ HeadRowsArgs a) {
+__global__ void __launch_bounds__(256, ROUNDS == 4 ? 4 : 5) head_rows_kernel(const __grid_constant__ HeadRowsArgs a) {
   constexpr int L = D / 8;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -98,16 +103,20 @@ __global__ void __launch_bounds__(256, ROUNDS == 1 ? 4 : 5) head_rows_kernel(con
   const bool rot = a.table != nullptr && 4 * j < a.half_rot;  // this lane's pairs turn, where the row does
   const bool split = rot && !a.interleaved;                   // and lie half_rot apart
 
-  // A row that does not exist (its lanes stay: the rows of a warp reduce together) reads the last one.
+  // A row that does not exist (its lanes stay: the rows of a warp reduce together) reads the last one. Rows and heads are few: where
+  // one lies in its token is 32-bit arithmetic, where the token lies is worked out once.
+  constexpr int XB = X == TURQ_F32 ? 4 : 2;
+  const uint8_t* const qp = static_cast<const uint8_t*>(a.q) + token * a.q_stride * XB;
+  const uint8_t* const kp = static_cast<const uint8_t*>(a.k) + token * a.k_stride * XB - (int64_t)a.hq * D * XB;
+  const uint8_t* const vp = static_cast<const uint8_t*>(a.v) + token * a.v_stride * XB - (int64_t)(a.hq + a.hkv) * D * XB;
   float x[ROUNDS][8];
 #pragma unroll
   for (int u = 0; u < ROUNDS; u++) {
     const int r = min(first + u * groups, rows - 1);
     const bool is_q = r < a.hq, is_v = r >= a.hq + a.hkv, apart = split && !is_v;
-    const int64_t base = is_q ? token * a.q_stride + r * D : is_v ? token * a.v_stride + (r - a.hq - a.hkv) * D : token * a.k_stride + (r - a.hq) * D;
-    const void* src = is_q ? a.q : is_v ? a.v : a.k;
-    load4(src, X, base + (apart ? 4 * j : 8 * j), reinterpret_cast<float(&)[4]>(x[u][0]));
-    load4(src, X, base + (apart ? a.half_rot + 4 * j : 8 * j + 4), reinterpret_cast<float(&)[4]>(x[u][4]));
+    const uint8_t* const src = is_q ? qp : is_v ? vp : kp;
+    load4(src, X, r * D + (apart ? 4 * j : 8 * j), reinterpret_cast<float(&)[4]>(x[u][0]));
+    load4(src, X, r * D + (apart ? a.half_rot + 4 * j : 8 * j + 4), reinterpret_cast<float(&)[4]>(x[u][4]));
   }
   const int64_t slot = a.slots ? a.slots[token] : -1;
   bool known = true;
@@ -128,6 +137,10 @@ __global__ void __launch_bounds__(256, ROUNDS == 1 ? 4 : 5) head_rows_kernel(con
   const bool write = KIND != ROWS_DENSE && slot >= 0 && fits && known;
   const int64_t row0 = write ? a.cache.row(slot, 0) : 0;  // of the planes; a page's heads are page_size rows apart
 
+  const int out_bytes = a.out_dtype == TURQ_F32 ? 4 : 2;
+  uint8_t* const qo = static_cast<uint8_t*>(a.q_out) + token * a.hq * D * out_bytes;
+  uint8_t* const ko = static_cast<uint8_t*>(a.k_out) + (token * a.hkv - a.hq) * D * out_bytes;
+
 #pragma unroll
   for (int u = 0; u < ROUNDS; u++) {
     const int r = first + u * groups;
@@ -139,7 +152,7 @@ __global__ void __launch_bounds__(256, ROUNDS == 1 ? 4 : 5) head_rows_kernel(con
       for (int e = 0; e < 8; e++) ss += y[e] * y[e];
 #pragma unroll
       for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-      const float inv = 1.f / sqrtf(ss / D + a.eps);
+      const float inv = inverse_root(ss / D + a.eps);
       const float* const w = is_q ? a.wq : is_v ? nullptr : a.wk;
       if (w) {
         float wv[8];
@@ -172,10 +185,9 @@ __global__ void __launch_bounds__(256, ROUNDS == 1 ? 4 : 5) head_rows_kernel(con
     }
     const int o0 = split && !is_v ? 4 * j : 8 * j, o1 = split && !is_v ? a.half_rot + 4 * j : 8 * j + 4;
     if (live && (is_q || KIND == ROWS_DENSE)) {
-      void* out = is_q ? a.q_out : a.k_out;
-      const int64_t o = is_q ? (token * a.hq + r) * D : (token * a.hkv + r - a.hq) * D;
-      store4(out, a.out_dtype, o + o0, y);
-      store4(out, a.out_dtype, o + o1, y + 4);
+      uint8_t* const out = is_q ? qo : ko;
+      store4(out, a.out_dtype, r * D + o0, y);
+      store4(out, a.out_dtype, r * D + o1, y + 4);
     }
     if (KIND == ROWS_DENSE) continue;
     const int h = is_v ? r - a.hq - a.hkv : r - a.hq;
