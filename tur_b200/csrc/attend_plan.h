@@ -36,12 +36,13 @@ TQ_HD int64_t keys_seen(const Span& s, int64_t t, bool causal) {
 
 // ---- single tokens: up to TOKEN_ROWS rows (new tokens x query heads of a key head)
 constexpr int TOKEN_ROWS = 16;
-// The contexts of a call are cut into chunks of one length, a CTA each, three or four CTAs at a time on an SM. A CTA has
-// costs of its own (the way from the lengths over the page table to the first keys, the join of its warps) worth
-// TOKEN_OVERHEAD keys, and 1 to 4 CTAs at a time on an SM take TOKEN_DEPTH times as long as the keys of one of them would if they did
-// not share it; a wave that is not the only one costs a full one. The length with the least cost is taken. Measured, us (8 heads of 128): one user at 16384 keys in bf16 in chunks of 256 18.4, 512 13.1, 1024 17.3; 24 users at 4096
-// 256 81, 1024 70, 2048 70; two at 120000 1024 156, 4480 148.
-constexpr int TOKEN_STEP = 128, TOKEN_CHUNK_MAX = 8192, TOKEN_OVERHEAD = 96;
+// The contexts of a call are cut into chunks of one length, a CTA each, three or four CTAs at a time on an SM. A CTA has costs of its
+// own (the way from the lengths over the page table to the first keys, the join of its warps) worth TOKEN_OVERHEAD keys, and 1 to 4 CTAs
+// at a time on an SM take TOKEN_DEPTH times as long as the keys of one of them would if they did not share it; a wave that is not the
+// only one costs a full one. The length with the least cost is taken, over several waves at most TOKEN_CHUNK_WAVES: sequences differ, and
+// the longest should not end alone. Measured, us: one user at 16384 keys (32 heads on 8 of 128, bf16) in chunks of 256 18.4, 512 13.1,
+// 1024 17.3; 24 users at 4096 256 81, 1024 70, 2048 70; two at 120000 1024 156, 4480 148; one at 30000 and 31 at 500 2560 42, 6016 77.
+constexpr int TOKEN_STEP = 128, TOKEN_CHUNK_MAX = 8192, TOKEN_CHUNK_WAVES = 3200, TOKEN_OVERHEAD = 96;
 constexpr int TOKEN_DEPTH[5] = {0, 140, 162, 216, 264};  // hundredths
 constexpr int token_ctas(bool q8, bool eight_rows) { return q8 && eight_rows ? 4 : 3; }
 inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64_t max_context, int sms, int ctas) {
@@ -50,7 +51,7 @@ inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64
     const int64_t chunks = max_context <= c ? 1 : (max_context + c - 1) / c, n = pairs * chunks, slots = (int64_t)ctas * sms;
     const int64_t keys = c < max_context ? c : max_context, deep = (n + sms - 1) / sms;
     const int64_t t = (n > slots ? (n + slots - 1) / slots * TOKEN_DEPTH[ctas] : TOKEN_DEPTH[deep]) * (keys + TOKEN_OVERHEAD);
-    if (cost < 0 || t < cost) {
+    if (cost < 0 || (t < cost && (n <= slots || c <= TOKEN_CHUNK_WAVES))) {
       cost = t;
       best = c;
     }
