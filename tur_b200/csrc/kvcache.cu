@@ -4,8 +4,9 @@
 //     32: a position of 1e5 is known to 4e-3 of a turn's radian there);
 //   * head_rows_kernel: one pass over the rows of q, k and v. A row is one head of one token; x / sqrt(mean(x^2)
 //     + eps) * w and the rotation are done in registers, and the row goes to a dense tensor or to its page,
-//     rounded once or quantized to Q8_0;
-//   * kv_read_kernel: slots back into dense rows.
+//     rounded once or quantized to Q8_0. Every byte is read and written once; for many tokens the issue slots bound it (8192 tokens of
+//     40 f32 heads of 128 to bf16: 49 us, 5.1 TB/s, 69% of the slots taken), for few the way through memory (one token 2 us);
+//   * kv_read_kernel: slots back into dense rows (4099 tokens of 16 Q8_0 heads of 128 to f32 11 us, 3.9 TB/s).
 #include <new>
 
 #include "../../include/turq.h"
@@ -283,8 +284,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvPages c, const int
 }
 
 // Lanes for all rows of a token, 256 at most. Rounds: one where a call has so few tokens that blocks are what it lacks; otherwise two,
-// or four where a token has many wide rows (us, 1 / 2 / 4 rounds: 8192 tokens of 40 f32 rows of 128 64 / 69 / 53, 4099 of 16 bf16
-// rows of 128 11.8 / 11.0 / 12.8, 2049 of 60 bf16 rows of 64 11.0 / 10.4 / 11.3).
+// or four where a token has many wide rows (us, 1 / 2 / 4 rounds: 64 tokens of 80 f32 rows of 128 2.6 / 2.7 / 3.3, 8192 of 40 69 / 64 /
+// 49, 4099 of 16 bf16 rows of 128 into Q8_0 12.0 / 10.3 / 10.5, 2049 of 60 bf16 rows of 64 10.5 / 8.4 / 8.4).
 struct RowGrid { dim3 grid, block; int rounds; };
 static RowGrid plan_rows(int64_t n_tokens, int rows, int head_dim, int most = 4) {
   const int lanes = head_dim / 8;
