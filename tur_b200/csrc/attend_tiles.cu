@@ -7,12 +7,13 @@
 //   * warps 12..15  Q8_0 only: int8 tiles and their scales -> f16 operand tiles;
 //   * warp 8        one lane issues tcgen05.mma: S_t = Q_t K^T (both from shared memory), O_t += P_t V (P from TMEM);
 //   * warps 0..3 and 4..7  softmax of tile 0 and of tile 1, a thread per row: S from TMEM, running maximum and sum in
-//                   registers, P back into S's columns, and the division at the end. The two tiles take turns: while
-//                   the tensor core works on one the other's weights are computed.
+//                   registers, P back into S's columns (head dimension 64: into columns of its own, so that the next S
+//                   need not wait for the product), and the division at the end. The two tiles take turns at the
+//                   exponentials: while one's are computed the tensor core works on the other.
 // O is rescaled only where a row's maximum grew by more than 2^8 (weights and their sum then stay within f16 and
 // f32, and the quotient is the same); a thread owns its row, so that costs the warp that needs it 2 x D columns of TMEM.
-// Rows to TMEM lanes: softmax thread r of a tile is lane r. Order of the MMAs: PV of a tile is issued before the
-// next S of that tile, whose columns hold P, and a commit covers all MMAs before it: a full S says that O is complete.
+// Rows to TMEM lanes: softmax thread r of a tile is lane r. Order of the MMAs, where P shares S's columns: PV of a tile is
+// issued before the next S of that tile, and a commit covers all MMAs before it: a full S says that O is complete.
 #include "attend.cuh"
 #include "attend_launch.h"
 #include "tc_common.cuh"
@@ -300,7 +301,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
     row_at[t][r] = live ? rt | (r - rt * a.group) << 8 : -1;  // once, and not for every 16 bytes that come or go
     tile_sync(1 + t);
     float mul = a.scale_log2;
-    // Q into the operand layout, D / 8 lanes a row (a row a thread, every load would touch 32 lines: 7500 cycles against 1500); on f16
+    // Q into the operand layout, D / 8 lanes a row (a row a thread, every load would touch 32 lines: 7300 cycles against 3500); on f16
     // caches a bf16 row by the power of two that its largest element fits.
     if (t < tiles) {
       constexpr int L = D / 8, ROWS = TILE_M / L;  // rows of a pass
@@ -462,7 +463,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = at < 0 ? -1 : out0 + ((int64_t)(at & 255) * a.hq + (at >> 8)) * D;
         }
       }
-      // Rows go out through shared memory, a warp whole rows, for the same reason as Q comes in so (6500 cycles against 1500): through this
+      // Rows go out through shared memory, a warp whole rows, for the same reason as Q comes in so (6400 cycles against 3500): through this
       // tile's part of Q, which nothing reads any more, in one go or in two for 32 bits.
       const bool wide = pieces || a.out_dtype == TURQ_F32;
       const uint32_t stage = sQ + t * OP;
