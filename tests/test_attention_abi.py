@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 
+import tur_b200 as tq
 from tur_b200 import _lib
 from tur_b200.build import build
 
@@ -43,3 +44,12 @@ def test_null_arguments_are_rejected_not_dereferenced(lib):
     assert lib.turq_kv_write(None, None, None, 0, None, 0, 0, 1, None, None) == 1
     assert lib.turq_kv_read(None, None, None, 1, 0, None, None, None) == 1
     assert lib.turq_kv_attention(None, None, None, 0, 1, 1, 1, None, None, None, 1, 1, 1, 1, 1.0, 1, 1, None, None, 0, None) == 1
+
+
+@pytest.mark.parametrize("kwargs", [{"base": 1.0}, {"base": 0.0}, {"base": -2.0}, {"base": float("nan")}, {"base": float("inf")},
+                                    {"scaling": {"type": "linear", "factor": 0.5}}, {"scaling": {"type": "linear", "factor": float("nan")}},
+                                    {"scaling": {"type": "yarn", "factor": float("inf"), "original": 100}}, {"scaling": {"type": "yarn", "factor": 2.0}},
+                                    {"scaling": {"type": "yarn", "factor": 2.0, "original": 0}}, {"scaling": {"type": "other"}}])
+def test_tables_that_no_model_has(kwargs):
+    with pytest.raises(tq.TurqError):
+        tq.RotaryTable.new(64, 16, **kwargs)

@@ -12,6 +12,7 @@ Attention, per element, with w the exact softmax weights and A = sum_j w_j |v_j|
   their sum; keys and values of Q8_0; outputs) is off by up to 2^-25 however small it is. That adds 2^-25 sum_j |v_j|
   for the weights, 2^-25 for the values, 2^-25 for the output and scale 2^-25 sum |q| to a score.
 """
+import ctypes
 import math
 
 import numpy as np
@@ -19,6 +20,7 @@ import pytest
 import torch
 
 import tur_b200 as tq
+from tur_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -571,3 +573,91 @@ def test_a_layers_attention_token_by_token_and_at_once(tmp_path):
             got = torch.cat([step(cache, a, b, pages) for a, b in zip(cuts, cuts[1:])]).double()
             assert ((got - want).norm() / want.norm()).item() < 2.0 ** -6, (dtype, cuts)
     tq.context().poll_status()
+
+
+# ---- calls at the edges of what the header allows
+
+@pytest.mark.parametrize("kind,q_dtype", TYPES)
+@pytest.mark.parametrize("new,ctx", [(1, 300), (1, 3000), (1, 40000), (40, 40), (40, 9000), (300, 300)])
+def test_the_output_may_be_the_query(kind, q_dtype, new, ctx):
+    cache, table, q, starts, contexts, _, _ = make_case(31, [(new, ctx), (1, 70)], kind, q_dtype, 8, 2, 128, 64)
+    want = cache.attend(q, starts, contexts, table)
+    same = q.clone()
+    assert cache.attend(same, starts, contexts, table, out=same).data_ptr() == same.data_ptr()
+    assert torch.equal(same, want)
+    tq.context().poll_status()
+
+
+@pytest.mark.parametrize("kind", [torch.float16, "q8_0"])
+@pytest.mark.parametrize("new", [1, 2, 40])
+@pytest.mark.parametrize("exponent", [118, 126, -120])
+def test_queries_far_outside_the_range_of_f16(kind, new, exponent):
+    # q = +-2^e: divided by its row's power of two it is +-1. At 2^118 the key whose signs it has gets all of the weight (its score leads
+    # by 2^118 / sqrt(128) times tens): its values come out as they are. At 2^126 scale brings the score back into f32's range. At 2^-120
+    # all scores are 0 within 2^-110: the mean of the keys that a row sees.
+    d, ctx = 128, 200
+    g = gen(32)
+    cache = tq.KvCache.new(GT[kind], 4, 64, 1, d)
+    k, v = randn(g, ctx, 1, d), randn(g, ctx, 1, d)
+    slots = torch.arange(ctx, device="cuda")
+    cache.write(k, v, slots)
+    kc, vc = cache.read(slots)
+    best = 7
+    q = (torch.where(k[best, 0] < 0, -1.0, 1.0) * 2.0 ** exponent).to(torch.bfloat16).expand(new, 1, d).contiguous()
+    starts, contexts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, new], [ctx]))
+    got = cache.attend(q, starts, contexts, torch.arange(4, dtype=torch.int32, device="cuda")[None], out_dtype=torch.float32,
+                       scale=2.0 ** -20 if exponent == 126 else None)
+    if exponent > 0:
+        scores = (kc[:, 0].double() * torch.sign(q[0, 0].double())).sum(1)
+        assert scores.argmax() == best and scores[best] - scores[scores < scores[best]].max() > 1  # of f32 steps below 2^-16: all of the weight
+        assert torch.equal(got, vc[best].half().float().expand(new, 1, d))  # values of Q8_0 go into the product as f16, those of f16 are
+    else:
+        vd = vc[:, 0].double()
+        for t in range(new):
+            seen = vd[:ctx - new + t + 1]
+            # weights are exactly 1, values have 11 bits (Q8_0: rounded to f16), sums and quotient are f32's
+            tol = (2.0 ** -11 * (kind == "q8_0") + 2.0 ** -15) * seen.abs().mean(0) + 2.0 ** -25
+            assert ((got[t, 0].double() - seen.mean(0)).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_no_context_at_all_gives_zeros(new):
+    cache = tq.KvCache.new(tq.GgmlDType.BF16, 1, 16, 2, 64)
+    starts, contexts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, new], [0]))
+    q = torch.ones(new, 4, 64, dtype=torch.bfloat16, device="cuda")
+    got = cache.attend(q, starts, contexts, torch.empty(1, 0, dtype=torch.int32, device="cuda"))
+    assert not got.any()
+    tq.context().poll_status()
+
+
+def test_a_cache_that_owns_its_memory_and_a_workspace_too_small():
+    lib, ctx = _lib.load(), tq.context()
+    h = ctypes.c_void_p()
+    ctx.check(lib.turq_kv_cache_create(ctx.handle, int(tq.GgmlDType.F16), 600, 16, 1, 64, None, 0, ctypes.byref(h)))
+    s = torch.cuda.current_stream().cuda_stream
+    try:
+        memory, off = ctypes.c_void_p(), (ctypes.c_int64 * 4)()
+        ctx.check(lib.turq_kv_cache_layout(h, ctypes.byref(memory), off))
+        assert memory.value and off[0] == 0 and off[1] == 600 * 16 * 64 * 2
+        slots = torch.arange(600 * 16, device="cuda")
+        k, v = (torch.full((600 * 16, 1, 64), 7.0, device="cuda") for _ in range(2))
+        ctx.check(lib.turq_kv_read(ctx.handle, h, slots.data_ptr(), 600 * 16, 0, k.data_ptr(), v.data_ptr(), s))
+        assert not k.any() and not v.any()
+        q = torch.ones(1, 1, 64, dtype=torch.float16, device="cuda")
+        starts, contexts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 1], [9600]))
+        table = torch.arange(600, dtype=torch.int32, device="cuda")
+        nbytes = lib.turq_kv_attention_workspace(h, 1, 1, 1, 1, 9600)
+        assert nbytes > 0
+        ws, y = torch.empty(nbytes, dtype=torch.uint8, device="cuda"), torch.full((1, 1, 64), 5.0, device="cuda")
+        call = lambda p, n, scale=0.125: lib.turq_kv_attention(ctx.handle, h, q.data_ptr(), 64, 1, 1, 1, starts.data_ptr(), contexts.data_ptr(), table.data_ptr(),
+                                                               600, 1, 1, 9600, scale, 1, 0, y.data_ptr(), p, n, s)
+        assert call(ws.data_ptr(), nbytes - 1) == 2 and call(None, 0) == 2 and call(None, nbytes) == 1 and call(ws.data_ptr() + 8, nbytes) != 0
+        assert call(ws.data_ptr(), nbytes, 3e38) == 1 and call(ws.data_ptr(), nbytes, float("nan")) == 1
+        torch.cuda.synchronize()
+        assert (y == 5).all()
+        ctx.check(call(ws.data_ptr(), nbytes))
+        torch.cuda.synchronize()
+        assert not y.any()
+    finally:
+        torch.cuda.synchronize()
+        assert lib.turq_kv_cache_free(h) == 0

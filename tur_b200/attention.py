@@ -97,17 +97,21 @@ class RotaryTable:
         0.1 ln f + 1 (the YaRN paper's rule)."""
         if rotary_dim <= 0 or rotary_dim % 8:
             raise TurqError(2, f"rotary_dim {rotary_dim} must be a positive multiple of 8")
+        if not 1.0 < base < math.inf:
+            raise TurqError(1, f"base {base} must be finite and above 1")
         half = rotary_dim // 2
         freqs = [base ** (-2.0 * i / rotary_dim) for i in range(half)]
         scale = 1.0
         if scaling is not None:
             kind, factor = scaling.get("type"), float(scaling.get("factor", 1.0))
-            if factor < 1.0:
-                raise TurqError(1, f"scaling factor {factor} must be at least 1")
+            if not 1.0 <= factor < math.inf:
+                raise TurqError(1, f"scaling factor {factor} must be finite and at least 1")
             if kind == "linear":
                 freqs = [f / factor for f in freqs]
             elif kind == "yarn":
-                n = float(scaling["original"])
+                n = float(scaling.get("original", 0.0))
+                if not 0.0 < n < math.inf:
+                    raise TurqError(1, f"yarn scaling needs the original number of positions, got {scaling.get('original')}")
 
                 def pair_of(turns: float) -> float:
                     return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
@@ -278,7 +282,7 @@ class KvCache:
                out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """softmax(scale q K^T) V of the new tokens of n_seqs sequences over their pages: q [n, heads, d] packed, rows
         starts[i] .. starts[i + 1] (int32 [n_seqs + 1]) of sequence i, whose context of contexts[i] tokens (int32 [n_seqs], the new
-        ones last) lies in the pages page_table[i] (int32 [n_seqs, pages]). scale: 1 / sqrt(d) by default. Single tokens,
+        ones last) lies in the pages page_table[i] (int32 [n_seqs, pages]). scale: 1 / sqrt(d) by default. `out` may be q. Single tokens,
         chunks and whole prompts go together; max_new and max_context are the longest of each that the call may meet (the
         values on the device are not read here). `out` keeps its rows that belong to no sequence."""
         dev, d = self._device, self.head_dim

@@ -73,7 +73,7 @@ int32_t turq_kv_attention(turq_ctx* ctx, const turq_kv_cache* cache, const void*
     return api_fail(ctx, TURQ_E_SHAPE, "n_q_heads must be a multiple of the cache's heads, at most 128 to one");
   if (n_tokens < 0 || n_tokens > INT32_MAX / 2 || n_seqs < 0 || n_seqs > 65535 || hkv > 65535) return api_fail(ctx, TURQ_E_SHAPE, "n_tokens or n_seqs out of range");
   if (max_new < 0 || max_new > INT32_MAX / 2 || max_context < 0 || max_context > INT32_MAX / 2) return api_fail(ctx, TURQ_E_SHAPE, "max_new or max_context out of range");
-  if (!(scale > 0.f) || scale > FLT_MAX) return api_fail(ctx, TURQ_E_INVALID_ARG, "scale must be positive and finite");
+  if (!(scale > 0.f) || scale > FLT_MAX / 2.f) return api_fail(ctx, TURQ_E_INVALID_ARG, "scale must be positive and finite (below 2^127)");
   if (n_tokens == 0 || n_seqs == 0 || max_new == 0) return TURQ_OK;
   if (table_stride < (max_context + cache->page_size - 1) / cache->page_size)
     return api_fail(ctx, TURQ_E_SHAPE, "the page table has fewer pages a sequence than max_context needs");

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
         for (int p = 0; p < 2; p++) top = max(top, max(qf[j][s][p] & 0x7FFFu, (qf[j][s][p] >> 16) & 0x7FFFu));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const int e = min(max((int)(top >> 7) - 127, -100), 100);
+      const int e = min(max((int)(top >> 7) - 127, -126), 126);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
       f *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
