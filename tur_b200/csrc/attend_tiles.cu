@@ -4,7 +4,7 @@
 // side, so all rows share K and V) and walks the keys in tiles of 128:
 //   * warp 9        copies K and V tiles page by page by TMA into a ring (and prefetches the page table), and zeroes the
 //                   values behind the context's end (they may be anything, and 0 x NaN is NaN);
-//   * warps 12..15  Q8_0 only: int8 tiles and their scales -> f16 operand tiles;
+//   * warps 10..15  Q8_0 only: int8 tiles and their scales -> f16 operand tiles;
 //   * warp 8        one lane issues tcgen05.mma: S_t = Q_t K^T (both from shared memory), O_t += P_t V (P from TMEM);
 //   * warps 0..3 and 4..7  softmax of tile 0 and of tile 1, a thread per row: S from TMEM, running maximum and sum in
 //                   registers, P back into S's columns (head dimension 64: into columns of its own, so that the next S
@@ -23,12 +23,13 @@ namespace turq {
 
 constexpr int TILE_M = 128, TILE_N = 128;
 constexpr int POLY_OF = 8;
+constexpr int CONVERT = 192;  // threads that turn int8 into f16
 
 template <int D, bool Q8> struct TileGeomA {
   static constexpr int HALVES = D / 64;
   static constexpr int OPERAND = TILE_N * D * 2;      // a tile of K, V or Q: blocks of 64 columns, 128 rows of 128 bytes each
   static constexpr int STAGES = Q8 ? 3 : (D == 128 ? 4 : 8);
-  static constexpr int RAW = Q8 ? TILE_N * D + 1024 : 0;  // int8 rows, scales behind them
+  static constexpr int RAW = Q8 ? TILE_N * D + 1024 : 0;  // int8 rows, scales behind them (1024 bytes of alignment, TILE_N x D / 16 of scales)
   static constexpr int RAW_STAGES = Q8 ? 3 : 0;
   static constexpr int THREADS = Q8 ? 512 : 384;
   static constexpr int REG_SOFT = Q8 ? 192 : 208, REG_REST = Q8 ? 64 : 88;
@@ -77,10 +78,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint
 __device__ __forceinline__ void tile_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void tile_box2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 // The largest of three, one instruction.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -154,7 +151,7 @@ __device__ __forceinline__ void tile_sync(int id) { asm volatile("bar.sync %0, 1
 __device__ __forceinline__ void turn_wait(int id) { asm volatile("bar.sync %0, 256;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ void turn_give(int id) { asm volatile("bar.arrive %0, 256;" ::"r"(id) : "memory"); }
 
-struct TileMaps { CUtensorMap k, v, ks, vs; };
+struct TileMaps { CUtensorMap k, v; };
 
 struct Work {
   Span sp;
@@ -262,9 +259,9 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
 
   if (threadIdx.x == 32) {
     for (int i = 0; i < 2; i++) { bar_init(&q_full[i], 4); bar_init(&s_full[i], 1); bar_init(&p_full[i][0], 4); bar_init(&p_full[i][1], 4); bar_init(&s_read[i], 4); bar_init(&o_full[i], 1); }
-    for (int i = 0; i < ST; i++) { bar_init(&kv_full[i], Q8 ? 4 : 1); bar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < ST; i++) { bar_init(&kv_full[i], Q8 ? CONVERT / 32 : 1); bar_init(&kv_empty[i], 1); }
     bar_init(&v_fixed, 1);
-    for (int i = 0; i < 3; i++) { bar_init(&raw_full[i], 1); bar_init(&raw_empty[i], 4); }
+    for (int i = 0; i < 3; i++) { bar_init(&raw_full[i], 33); bar_init(&raw_empty[i], CONVERT / 32); }
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -609,7 +606,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
     } else if (warp == 9) {
       // -------------------------------------------------------------- copies
       // lane i: the page that key 16 i of the tile begins (boxes of a page's tokens, 16 to 128 of them)
-      const int box = min(a.cache.page_size, TILE_N), boxes = TILE_N / box;
+      const int box_shift = min(a.cache.page_shift, 7), box = 1 << box_shift, boxes = TILE_N >> box_shift;
       const int32_t* table = a.page_table + seq * a.table_stride;
       auto page_of = [&](int j) {  // z coordinate of this lane's box in key tile begin + j; -1: behind the context
         const int64_t key = (int64_t)(begin + j) * TILE_N + lane * box;
@@ -620,6 +617,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         return known ? (int)(p * a.cache.n_heads + head) : (int)(a.cache.n_pages * a.cache.n_heads);
       };
       int stage = 0, z = page_of(0);
+      const int pages_end = (int)(a.cache.n_pages * a.cache.n_heads);
       uint32_t ph = 0;
       for (int j = 0; j < n_iter; j++) {
         if (__any_sync(0xFFFFFFFFu, *abort_flag)) break;
@@ -641,19 +639,28 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           } else {
             tile_wait(&raw_empty[stage], ph ^ 1u, abort_flag);
             const uint32_t bar = s_u32(&raw_full[stage]), at = sRaw + stage * G::RAW;
-            if (lane == 0) bar_expect_tx(&raw_full[stage], n * box * (D + D / 16));
+            if (lane == 0) bar_expect_tx(&raw_full[stage], n * box * D);
             __syncwarp();
-            if (z >= 0) {
-              tile_box3(at + lane * box * D, kv ? &maps.v : &maps.k, 0, y, z, bar);
-              // scales: 16 keys' in 128 bytes each (of which D = 64 fills half), as copies ask for
-              for (int b = 0; b < box / 16; b++)
-                tile_box2(at + TILE_N * D + (lane * box / 16 + b) * 128, kv ? &maps.vs : &maps.ks, (y + 16 * b) * (D / 32), z, bar);
+            if (z >= 0) tile_box3(at + lane * box * D, kv ? &maps.v : &maps.k, 0, y, z, bar);
+            // Scales are too small for boxes (16 of 64 bytes a tile; with pages of 16 tokens head dimension 64 then waits for the copies' rate:
+            // one prompt of 8192 tokens 618 us, 541 this way): 16 bytes at a time, zeros where there is no page.
+            const __half* const from = kv ? a.cache.vs : a.cache.ks;
+#pragma unroll
+            for (int i = 0; i < D / 64; i++) {
+              constexpr int PER = 256 / D;  // keys whose scales are 16 bytes
+              const int key = (i * 32 + lane) * PER, zk = __shfl_sync(0xFFFFFFFFu, z, key >> box_shift);
+              const bool have = zk >= 0 && zk < pages_end;
+              const __half* const src = from + ((int64_t)(have ? zk : 0) * a.cache.page_size + (((begin + j) * TILE_N + key) & (a.cache.page_size - 1))) * (D / 32);
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sRaw + stage * G::RAW + TILE_N * D + key * (D / 16)), "l"(src), "r"(have ? 16 : 0)
+                           : "memory");
             }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
             if (++stage == G::RAW_STAGES) { stage = 0; ph ^= 1u; }
           }
         }
         z = z2;
       }
+      if (Q8) asm volatile("cp.async.wait_all;" ::: "memory");  // (after a wait that ran out: nothing is on its way when the block ends)
       // Values behind the context's end. Only this warp can wait for a phase of kv_full that is many on: it knows that the one
       // before is over, as its own wait for the empty stage said.
       if (!Q8 && n_iter > 0 && (begin + n_iter) * TILE_N > ctx) {
@@ -667,9 +674,9 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         __syncwarp();
         if (lane == 0) bar_arrive(&v_fixed);
       }
-    } else if (warp >= 12) {
+    } else if (Q8) {
       // -------------------------------------------------------------- int8 -> f16 operand tiles
-      const int id0 = threadIdx.x - 384;
+      const int id0 = threadIdx.x - 320;
       int rs = 0, stage = 0;
       uint32_t rp = 0, ph = 0;
       for (int j = 0; j < 2 * n_iter; j++) {
@@ -677,13 +684,14 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         tile_wait(&raw_full[rs], rp, abort_flag);
         tile_wait(&kv_empty[stage], ph ^ 1u, abort_flag);
         const uint32_t src = sRaw + rs * G::RAW, dst = sKV + stage * OP;
-#pragma unroll 4
-        for (int i = 0; i < D / 16; i++) {
-          const int id = i * 128 + id0, row = id / (D / 16), ch = id % (D / 16);
+#pragma unroll 3
+        for (int i = 0; i < (TILE_N * D / 16 + CONVERT - 1) / CONVERT; i++) {
+          const int id = i * CONVERT + id0, row = id / (D / 16), ch = id % (D / 16);
+          if (id >= TILE_N * D / 16) break;
           uint4 w;
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(src + id * 16));
           uint16_t sc;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc) : "r"(src + TILE_N * D + (row >> 4) * 128 + ((row & 15) * (D / 32) + (ch >> 1)) * 2));
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc) : "r"(src + TILE_N * D + (row * (D / 32) + (ch >> 1)) * 2));
           const __half2 scale = __half2half2(__ushort_as_half(sc)), off = __float2half2_rn(1152.f);
           const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
           uint32_t h[8];
@@ -775,7 +783,7 @@ static cudaError_t launch_tiles(const turq_kv_cache* kc, const AttendArgs& a, un
     if (e != cudaSuccess) return e;
     configured.set(dev);
   }
-  const TileMaps maps{kc->k_tile, kc->v_tile, kc->ks16, kc->vs16};
+  const TileMaps maps{kc->k_tile, kc->v_tile};
   return launch_pdl(attend_tiles_kernel<D, Q8, BF>, dim3(blocks), dim3(G::THREADS), G::SMEM, s, maps, a);
 }
 
