@@ -610,7 +610,10 @@ def test_queries_far_outside_the_range_of_f16(kind, new, exponent):
     if exponent > 0:
         scores = (kc[:, 0].double() * torch.sign(q[0, 0].double())).sum(1)
         assert scores.argmax() == best and scores[best] - scores[scores < scores[best]].max() > 1  # of f32 steps below 2^-16: all of the weight
-        assert torch.equal(got, vc[best].half().float().expand(new, 1, d))  # values of Q8_0 go into the product as f16, those of f16 are
+        # Values of Q8_0 go into the product as f16, those of f16 are. The row's one weight, some 2^r, is rounded to f16 for the product (2^-11 of
+        # it) and not for the sum that divides it; the f32 product and quotient add 2^-24 each.
+        want = vc[best].half().double()
+        assert ((got.double() - want).abs() <= (2.0 ** -11 + 2.0 ** -22) * want.abs()).all()
     else:
         vd = vc[:, 0].double()
         for t in range(new):
@@ -618,6 +621,28 @@ def test_queries_far_outside_the_range_of_f16(kind, new, exponent):
             # weights are exactly 1, values have 11 bits (Q8_0: rounded to f16), sums and quotient are f32's
             tol = (2.0 ** -11 * (kind == "q8_0") + 2.0 ** -15) * seen.abs().mean(0) + 2.0 ** -25
             assert ((got[t, 0].double() - seen.mean(0)).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind,q_dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), ("q8_0", torch.bfloat16)])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_that_climb_back_from_far_below(kind, q_dtype, new, d):
+    # The first 128 keys point away from every query: scores below -2^22, weights of exactly 0 once an ordinary key is seen. What a row gives is
+    # attention over the other 200 alone.
+    g = gen(33)
+    ctx, far = 328, 128
+    cache = tq.KvCache.new(GT[kind], 6, 64, 1, d)
+    base = randn(g, 1, 1, d).sign()
+    q = (base * (3 + randn(g, new, 1, d).abs())).to(q_dtype)
+    k, v = 0.05 * randn(g, ctx, 1, d), randn(g, ctx, 1, d)
+    k[:far] = -50000.0 * base
+    slots = torch.arange(ctx, device="cuda")
+    cache.write(k, v, slots)
+    kc, vc = cache.read(slots)
+    assert ((q.double() * kc[:1].double()).sum(-1) < -2.0 ** 22).all()
+    starts, contexts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, new], [ctx]))
+    got = cache.attend(q, starts, contexts, torch.arange(6, dtype=torch.int32, device="cuda")[None], scale=1.0)
+    check_attention(got, q, kc[far:], vc[far:], [(new, ctx - far)], kind=kind, scale=1.0)
 
 
 @pytest.mark.parametrize("new", [1, 30])

@@ -297,7 +297,6 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
     const bool live = rt < tpt && tok < sp.n;
     row_at[t][r] = live ? rt | (r - rt * a.group) << 8 : -1;  // once, and not for every 16 bytes that come or go
     tile_sync(1 + t);
-    float mul = a.scale_log2;
     // Q into the operand layout, D / 8 lanes a row (a row a thread, every load would touch 32 lines: 7300 cycles against 3500); on f16
     // caches a bf16 row by the power of two that its largest element fits.
     if (t < tiles) {
@@ -333,11 +332,10 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) bar_arrive(&q_full[t]);
-      if (convert) {
-        tile_sync(1 + t);
-        mul *= row_up[t][r];
-      }
+      if (convert) tile_sync(1 + t);
     }
+    auto true_mul = [&] { return !BF && a.q_bf16 ? a.scale_log2 * row_up[t][r] : a.scale_log2; };
+    float mul = a.scale_log2;
     const int seen = live ? (int)min(sp.ctx, keys_seen(sp, tok, a.causal)) : INT32_MAX;  // rows that do not exist ask for no mask
     // keys that every row of the warp sees
     int least = seen;
@@ -346,7 +344,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in the address' upper half
     const uint32_t tS = tmem + lanes + COL_S + 128 * t, tO = tmem + lanes + COL_O + D * t, tP = APART ? tmem + lanes + COL_P + 64 * t : tS;
     float m = -INFINITY, l = 0.f;  // maximum in units of S, as last subtracted; sum of the weights
-    const float lag = 8.f / mul;
+    float above = 0.f, sub = 0.f;  // maxima above this one are taken over: their weights would be 2^8 and more; maximum x mul
     if (t >= tiles && work.splits > 1 && work.split == 0) a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = -1;
     if (t < tiles) {
       if (tiles == 2 && t == 1 && n_iter > 0) turn_give(3);
@@ -383,36 +381,39 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         }
         largest(64);
         const float mt = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-        if (j == 0) {
-          m = mt;
-        } else if (__any_sync(0xFFFFFFFFu, mt > m + lag)) {
-          if (APART) {  // otherwise a full S says so
-            tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
-            tc_after();
-          }
-          const float m2 = fmaxf(m, mt), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * mul);  // m = -inf: 0 of nothing
-          m = m2;
-          l *= f;
-          float o[16];
+        if (j == 0 || __any_sync(0xFFFFFFFFu, mt > above)) {
+          if (j == 0) {
+            m = mt;
+          } else {
+            if (APART) {  // otherwise a full S says so
+              tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
+              tc_after();
+            }
+            const float m2 = fmaxf(m, mt), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * true_mul());  // m = -inf: 0 of nothing
+            m = m2;
+            l *= f;
+            float o[16];
 #pragma unroll 1
-          for (int i = 0; i < D / 16; i++) {
-            tmem_ld16(o, tO + 16 * i);
-            tmem_wait_ld();
+            for (int i = 0; i < D / 16; i++) {
+              tmem_ld16(o, tO + 16 * i);
+              tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[e] *= f;
-            tmem_st16(tO + 16 * i, reinterpret_cast<const uint32_t*>(o));
+              for (int e = 0; e < 16; e++) o[e] *= f;
+              tmem_st16(tO + 16 * i, reinterpret_cast<const uint32_t*>(o));
+            }
+            tmem_wait_st();
           }
-          tmem_wait_st();
-        }
-        float sub = m == -INFINITY ? 0.f : m * mul;
-        // Every exponent below is off by what m x mul lost in rounding, the same for all weights of a row, so that it cancels in the quotient.
-        // Above 2^22 it may be more than 1/4, and from 2^27 on weights would leave f16: such scores are taken relative to m first.
-        // (The question costs 1 to 2% of a long prompt; asked only where m changes, 6% at head dimension 64.)
-        if (__builtin_expect(__any_sync(0xFFFFFFFFu, fabsf(sub) > 4194304.f), 0)) {
-          const float mm = m == -INFINITY ? 0.f : m;
-#pragma unroll
-          for (int i = 0; i < TILE_N; i++) s[i] -= mm;
-          sub = 0.f;
+          // Every exponent is off by what m x mul loses in rounding: the same for all weights of a row, so that it cancels in the quotient,
+          // but from 2^27 on f16 weights would leave their range. There a step of an f32 score is itself 2^3, and its sum of D products is
+          // good to D / 2 of them: a row beyond 2^22 takes mul for as much as makes it 2^22, which moves weights by less than that (keys
+          // further off than the scores' error have 2^-16 and less either way). From the true mul, as m may have come from far below.
+          mul = true_mul();
+          sub = m == -INFINITY ? 0.f : m * mul;
+          if (fabsf(sub) > 4194304.f) {
+            mul = 4194304.f / fabsf(m);
+            sub = m * mul;
+          }
+          above = m + 8.f / mul;
         }
         if (APART && j > 0) {  // the last weights' product has read them
           tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
@@ -463,7 +464,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       const int64_t piece0 = (int64_t)blockIdx.x * (2 * TILE_M) + TILE_M * t;
       const int64_t out0 = ((work.sp.first + work.tok0 + t * tpt) * a.hq + work.head * a.group) * D;  // of the tile's first row
       if (pieces) {
-        a.tile_ml[piece0 + r] = make_float2(m * mul, l);
+        a.tile_ml[piece0 + r] = make_float2(m * true_mul(), l);
         if (work.split == 0) {
           const int at = row_at[t][r];
           a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = at < 0 ? -1 : out0 + ((int64_t)(at & 255) * a.hq + (at >> 8)) * D;
