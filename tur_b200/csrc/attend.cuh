@@ -49,6 +49,18 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Scores are compared and subtracted as the products gave them, and multiplied (by scale x log2 e, times what a row of q was divided by)
+// afterwards: the product of a large score would be off by its own f32 rounding, in every weight a different one. Where pieces of a row meet,
+// their maxima come times the power of two in the row's multiplier, which is exact, and what is left of it, from 1 to 2, is the same for
+// all rows: a weight is 2^((maximum - largest) * joined_factor).
+__device__ __forceinline__ float row_mul(const AttendArgs& a, float up) {
+  return fmaxf(a.scale_log2 * up, __uint_as_float(1u));  // not zero: the score of a key that is not seen is -inf
+}
+__device__ __forceinline__ float joined_max(float m, float mul) {
+  return m == -INFINITY ? m : m * __uint_as_float(__float_as_uint(mul) & 0x7F800000u);
+}
+__device__ __forceinline__ float joined_factor(const AttendArgs& a) { return __uint_as_float((__float_as_uint(a.scale_log2) & 0x7FFFFFu) | 0x3F800000u); }
+
 // Two neighbouring elements of the output, rounded once.
 __device__ __forceinline__ void store_out2(void* out, int dtype, int64_t i, float a, float b) {
   if (dtype == TURQ_F32) *reinterpret_cast<float2*>(static_cast<float*>(out) + i) = make_float2(a, b);

@@ -334,8 +334,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       if (lane == 0) bar_arrive(&q_full[t]);
       if (convert) tile_sync(1 + t);
     }
-    auto true_mul = [&] { return !BF && a.q_bf16 ? a.scale_log2 * row_up[t][r] : a.scale_log2; };
-    float mul = a.scale_log2;
+    const float mul = !BF && a.q_bf16 && t < tiles ? row_mul(a, row_up[t][r]) : a.scale_log2;
     const int seen = live ? (int)min(sp.ctx, keys_seen(sp, tok, a.causal)) : INT32_MAX;  // rows that do not exist ask for no mask
     // keys that every row of the warp sees
     int least = seen;
@@ -389,7 +388,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
               tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
               tc_after();
             }
-            const float m2 = fmaxf(m, mt), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * true_mul());  // m = -inf: 0 of nothing
+            const float m2 = fmaxf(m, mt), f = m2 == -INFINITY ? 1.f : ex2((m - m2) * mul);  // m = -inf: 0 of nothing
             m = m2;
             l *= f;
             float o[16];
@@ -403,21 +402,23 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
             }
             tmem_wait_st();
           }
-          // Every exponent is off by what m x mul loses in rounding: the same for all weights of a row, so that it cancels in the quotient,
-          // but from 2^27 on f16 weights would leave their range. There a step of an f32 score is itself 2^3, and its sum of D products is
-          // good to D / 2 of them: a row beyond 2^22 takes mul for as much as makes it 2^22, which moves weights by less than that (keys
-          // further off than the scores' error have 2^-16 and less either way). From the true mul, as m may have come from far below.
-          mul = true_mul();
+          // A weight's exponent is one FMA, s x mul - sub: off by what m x mul loses in rounding, the same for all weights until m changes. From
+          // 2^10 on that is 2^-14 and more: such rows (above = m says so) subtract m from their scores before they multiply.
           sub = m == -INFINITY ? 0.f : m * mul;
-          if (fabsf(sub) > 4194304.f) {
-            mul = 4194304.f / fabsf(m);
-            sub = m * mul;
-          }
           above = m + 8.f / mul;
+          if (fabsf(sub) > 1024.f) {
+            sub = 0.f;
+            above = m;
+          }
         }
         if (APART && j > 0) {  // the last weights' product has read them
           tile_wait(&o_full[t], (j - 1) & 1, abort_flag);
           tc_after();
+        }
+        if (above == m) {  // (or no key seen yet)
+          const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int i = 0; i < TILE_N; i++) s[i] -= mm;
         }
         // The tiles take turns at the exponentials, which one warp a scheduler can keep busy: together both would take as long as one behind
         // the other, and then both wait for the tensor core at once.
@@ -464,7 +465,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       const int64_t piece0 = (int64_t)blockIdx.x * (2 * TILE_M) + TILE_M * t;
       const int64_t out0 = ((work.sp.first + work.tok0 + t * tpt) * a.hq + work.head * a.group) * D;  // of the tile's first row
       if (pieces) {
-        a.tile_ml[piece0 + r] = make_float2(m * true_mul(), l);
+        a.tile_ml[piece0 + r] = make_float2(joined_max(m, mul), l);
         if (work.split == 0) {
           const int at = row_at[t][r];
           a.tile_rows[(int64_t)work.id * (2 * TILE_M) + TILE_M * t + r] = at < 0 ? -1 : out0 + ((int64_t)(at & 255) * a.hq + (at >> 8)) * D;
@@ -753,7 +754,7 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(const __grid_constant__
     mm = mine.x;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, d));
-    const float f = mm == -INFINITY ? 0.f : ex2(mine.x - mm), fl = f * mine.y;
+    const float f = mm == -INFINITY ? 0.f : ex2((mine.x - mm) * joined_factor(a)), fl = f * mine.y;
 #pragma unroll 4
     for (int k = 0; k < splits; k++) {
       const float w = __shfl_sync(0xFFFFFFFFu, f, k);

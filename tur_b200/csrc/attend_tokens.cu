@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       const int e = min(max((int)(top >> 7) - 127, -126), 126);
       const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      f *= __uint_as_float((uint32_t)(127 + e) << 23);
+      f = row_mul(a, __uint_as_float((uint32_t)(127 + e) << 23));
 #pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -269,7 +269,6 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             float& x = s[kt][j][2 * h + e];
-            x *= mul[j][e];
             if (k0 + KEYS > least && k0 + 16 * kt + 8 * h + g >= seen[j][e]) x = -INFINITY;
             top[j][e] = fmaxf(top[j][e], x);
           }
@@ -285,7 +284,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
         float was[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          was[e] = m[j][e] == -INFINITY ? 0.f : ex2(m[j][e] - top[j][e]);
+          was[e] = m[j][e] == -INFINITY ? 0.f : ex2((m[j][e] - top[j][e]) * mul[j][e]);
           m[j][e] = top[j][e];
           l[j][e] *= was[e];
         }
@@ -305,7 +304,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
       for (int kt = 0; kt < KT; kt++) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const float x = ex2(s[kt][j][2 * h] - sub[0]), y = ex2(s[kt][j][2 * h + 1] - sub[1]);
+          const float x = ex2((s[kt][j][2 * h] - sub[0]) * mul[j][0]), y = ex2((s[kt][j][2 * h + 1] - sub[1]) * mul[j][1]);
           l[j][0] += x;
           l[j][1] += y;
           asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[kt][j][h]) : "r"(pack16<BF>(x, y)));
@@ -394,7 +393,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
         ro[row * G::RES + (Q8 ? D / 8 * g + 2 * i + 1 : 16 * i + g + 8)] = o[j][i][2 + e];
       }
       if (g == 0) {
-        rml[2 * row] = m[j][e];
+        rml[2 * row] = joined_max(m[j][e], mul[j][e]);
         rml[2 * row + 1] = l[j][e];
       }
     }
@@ -402,6 +401,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
   __syncthreads();
   const bool whole = sp.ctx <= a.chunk;
   const int64_t item = ((int64_t)seq * a.cache.n_heads + head) * a.max_chunks + chunk;
+  const float factor = joined_factor(a);
   const float* const rb = reinterpret_cast<const float*>(raw + (base - s_u32(raw)));
   // where a cluster's blocks leave their piece for one another: row r behind the result of warp r % 4
   const uint32_t left = base + 16 * G::RES * 4 + 128;
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
 #pragma unroll
     for (int w = 0; w < TOK_WARPS; w++) {
       const float* p = rb + w * (G::RING / 4);
-      const float f = mm == -INFINITY ? 0.f : ex2(p[16 * G::RES + 2 * r] - mm);
+      const float f = mm == -INFINITY ? 0.f : ex2((p[16 * G::RES + 2 * r] - mm) * factor);
       const float2 v = *reinterpret_cast<const float2*>(p + r * G::RES + d);
       ll += f * p[16 * G::RES + 2 * r + 1];
       x += f * v.x;
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
 #pragma unroll
       for (int k = 0; k < TOKEN_CLUSTER; k++) {
         if (k >= chunks) break;
-        const float f = mm == -INFINITY ? 0.f : ex2(ml[k].x - mm);
+        const float f = mm == -INFINITY ? 0.f : ex2((ml[k].x - mm) * factor);
         ll += f * ml[k].y;
         x += f * v[k].x;
         y += f * v[k].y;
@@ -488,14 +488,14 @@ __global__ void __launch_bounds__(256) join_tokens_kernel(const __grid_constant_
   for (int k = lane; k < chunks; k += 32) mm = fmaxf(mm, ml[(int64_t)k * a.part_rows].x);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, d));
-  const float sub = mm == -INFINITY ? 0.f : mm;
+  const float sub = mm == -INFINITY ? 0.f : mm, factor = joined_factor(a);
   float ll = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; e++) o[e] = 0.f;
 #pragma unroll 4
   for (int k = warp; k < chunks; k += WARPS) {
     const float2 t = ml[(int64_t)k * a.part_rows];
-    const float f = ex2(t.x - sub);
+    const float f = ex2((t.x - sub) * factor);
     ll += f * t.y;
     const float* p = po + (int64_t)k * a.part_rows * D;
 #pragma unroll
