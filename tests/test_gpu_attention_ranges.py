@@ -94,6 +94,60 @@ def test_scores_that_vanish_leave_the_mean(kind, new):
 
 @pytest.mark.parametrize("kind,q_dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", ["tokens", "tiles"])
+def test_a_key_that_is_not_a_number_is_seen_by_every_row_behind_it(kind, q_dtype, d, rows):
+    # Rows that see the key are NaN throughout, the others what they are without it; at every place that a key can have among the 32
+    # that a thread takes at a time, and at the ends of the tiles.
+    g = gen(42)
+    ctx, new = (200, 40) if rows == "tiles" else (200, 2)
+    cache, table = plain_cache(kind, ctx, d)
+    k, v, q = randn(g, ctx, 1, d), randn(g, ctx, 1, d), randn(g, new, 4, d).to(q_dtype)
+    slots = torch.arange(ctx, device="cuda")
+    cache.write(k, v, slots)
+    want = cache.attend(q, ints(0, new), ints(ctx), table)
+    assert torch.isfinite(want).all()
+    for at in list(range(32)) + [63, 64, 126, 127, 128, 129, ctx - new, ctx - 1]:
+        plane = cache.k_scales if kind == "q8_0" else cache.k_pages
+        old = plane[at // 64, 0, at % 64].clone()
+        plane[at // 64, 0, at % 64] = float("nan")
+        got = cache.attend(q, ints(0, new), ints(ctx), table)
+        plane[at // 64, 0, at % 64] = old
+        first = max(0, at - (ctx - new))  # the first row that sees it
+        assert torch.isnan(got[first:]).all(), at
+        assert torch.equal(got[:first], want[:first]), at
+    assert torch.equal(cache.attend(q, ints(0, new), ints(ctx), table), want)
+    cache_status()
+
+
+def cache_status():
+    try:
+        tq.context().poll_status()
+    except tq.TurqError:
+        pass
+
+
+@pytest.mark.parametrize("kind,q_dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [2, 40, 300])
+def test_values_that_a_row_does_not_see_have_no_weight(kind, q_dtype, d, new):
+    # every value is as large as its type goes, but for the first: the row that sees nothing else gives it. Its one weight, whatever the
+    # exponential makes of 0, is rounded to the 16-bit type for the product and not for the sum that divides it: half a step of it, and
+    # what f32 loses in product and quotient (2^-22 is four half steps).
+    g = gen(43)
+    ctx = new
+    cache, table = plain_cache(kind, ctx, d)
+    v = torch.full((ctx, 1, d), 3e38 if kind is torch.bfloat16 else 65504.0, device="cuda")
+    v[0] = randn(g, 1, d)
+    cache.write(torch.zeros(ctx, 1, d, device="cuda"), v, torch.arange(ctx, device="cuda"))
+    q = randn(g, new, 8, d).to(q_dtype)
+    got = cache.attend(q, ints(0, new), ints(ctx), table, out_dtype=torch.float32)
+    first = v[0].to(kind).float().expand(8, d)
+    assert ((got[0] - first).abs() <= (HALF[kind] + 2.0 ** -22) * first.abs()).all()
+    tq.context().poll_status()
+
+
+@pytest.mark.parametrize("kind,q_dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
 def test_maxima_that_grow_from_tile_to_tile(kind, q_dtype, d):
     """Every tile of 128 keys has scores far above the one before, so that sums and products are scaled again at each of them."""
     g = gen(44)

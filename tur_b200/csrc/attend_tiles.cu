@@ -102,13 +102,23 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // 2^x of two f32 on the FMA units: x = n + f with n the nearest whole number (Cody and Waite; adding 1.5 x 2^23 rounds), 2^f by the
-// polynomial of degree 3 that is off by least, relative, on [-1/2, 1/2] (2^-13.7; fitted by Remez' exchange), n into the exponent.
-// Below 2^-126 it stays there: what comes of -inf is not quite zero.
+// polynomial of degree 3 that is off by least, relative, on [-1/2, 1/2] (2^-13.7; fitted by Remez' exchange), times 2^n, whose exponent n + 127
+// the rounding leaves in the lowest bits. n = -127, where x is held, has the bits of zero: -inf gives 0. NaN stays.
+__device__ __forceinline__ float at_least(float x, float low) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
+  return r;
+}
 __device__ __forceinline__ void ex2_pair(uint64_t v, float& x, float& y) {
   un2(v, x, y);
-  const uint64_t big = f2(12582912.f, 12582912.f), less = f2(-12582912.f, -12582912.f), one = f2(-1.f, -1.f);
-  v = f2(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const uint64_t big = f2(12583039.f, 12583039.f), less = f2(-12583039.f, -12583039.f), one = f2(-1.f, -1.f);
+  v = f2(at_least(x, -127.f), at_least(y, -127.f));
   const uint64_t t = add2(v, big);
   const uint64_t f = fma2(add2(t, less), one, v);
   uint64_t p = fma2(f, f2(0.05517166852951050f, 0.05517166852951050f), f2(0.2426111251115799f, 0.2426111251115799f));
@@ -116,9 +126,7 @@ __device__ __forceinline__ void ex2_pair(uint64_t v, float& x, float& y) {
   p = fma2(p, f, f2(0.9999280571937561f, 0.9999280571937561f));
   float tx, ty;
   un2(t, tx, ty);
-  un2(p, x, y);
-  x = __int_as_float(__float_as_int(x) + (__float_as_int(tx) << 23));
-  y = __int_as_float(__float_as_int(y) + (__float_as_int(ty) << 23));
+  un2(mul2(p, f2(__int_as_float(__float_as_int(tx) << 23), __int_as_float(__float_as_int(ty) << 23))), x, y);
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pack_p(float a, float b) {
@@ -423,7 +431,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         // The tiles take turns at the exponentials, which one warp a scheduler can keep busy: together both would take as long as one behind
         // the other, and then both wait for the tensor core at once.
         if (tiles == 2) turn_wait(3 + t);
-        const uint64_t mul2 = f2(mul, mul), sub2 = f2(-sub, -sub);
+        const uint64_t times = f2(mul, mul), less = f2(-sub, -sub);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int h = 0; h < TILE_N / 32; h++) {
@@ -431,7 +439,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             float x, y;
-            const uint64_t e = fma2(f2(s[32 * h + 2 * i], s[32 * h + 2 * i + 1]), mul2, sub2);
+            const uint64_t e = fma2(f2(s[32 * h + 2 * i], s[32 * h + 2 * i + 1]), times, less);
             if (i % POLY_OF < POLY) {
               ex2_pair(e, x, y);
             } else {
