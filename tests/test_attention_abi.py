@@ -53,3 +53,24 @@ def test_null_arguments_are_rejected_not_dereferenced(lib):
 def test_tables_that_no_model_has(kwargs):
     with pytest.raises(tq.TurqError):
         tq.RotaryTable.new(64, 16, **kwargs)
+
+
+@pytest.mark.parametrize("dim,base,original,factor,ramp", [(64, 1e4, 65536, 8.0, (20, 33)), (128, 1e4, 131072, 4.0, (45, 70)), (64, 1e4, 2048, 4.0, (8, 21)),
+                                                           (128, 1e6, 32768, 4.0, (23, 40)), (16, 1e4, 10 ** 9, 2.0, (13, 15))])
+def test_yarn_blends_between_its_two_pairs(dim, base, original, factor, ramp, monkeypatch):
+    """The pairs that turn beta_fast = 32 and beta_slow = 1 times over the original positions, as numbers between pairs: rounded outwards and held
+    to 0 .. dim - 1, which lies behind the last pair (dim / 2 - 1). Frequencies go from kept to divided by the factor linearly in between."""
+    import math
+    for turns, end, rounded in ((32, ramp[0], math.floor), (1, ramp[1], math.ceil)):
+        # base^(-2 p / dim) * original = 2 pi turns
+        assert min(dim - 1, max(0, rounded(dim / 2 * math.log(original / (2 * math.pi * turns), base)))) == end
+    made = {}
+    monkeypatch.setattr(tq.RotaryTable, "from_frequencies", classmethod(lambda cls, freqs, n, interleaved, scale, device, ctx: made.update(freqs=freqs, scale=scale)))
+    tq.RotaryTable.new(dim, 16, base=base, scaling={"type": "yarn", "factor": factor, "original": original})
+    assert made["scale"] == pytest.approx(0.1 * math.log(factor) + 1, rel=1e-15) and len(made["freqs"]) == dim // 2
+    for i, f in enumerate(made["freqs"]):
+        kept = 1 - min(1.0, max(0.0, (i - ramp[0]) / (ramp[1] - ramp[0])))
+        plain = base ** (-2 * i / dim)
+        assert f == pytest.approx(plain * kept + plain / factor * (1 - kept), rel=1e-13), i
+        if plain * original > 2 * math.pi:  # more than one turn: not stretched all the way
+            assert f > plain / factor * (1 + 1e-9)

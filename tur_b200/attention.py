@@ -117,7 +117,7 @@ class RotaryTable:
                     return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
 
                 low = max(0, math.floor(pair_of(float(scaling.get("beta_fast", 32)))))
-                high = min(half - 1, math.ceil(pair_of(float(scaling.get("beta_slow", 1)))))
+                high = min(rotary_dim - 1, math.ceil(pair_of(float(scaling.get("beta_slow", 1)))))
                 for i in range(half):
                     slow = min(1.0, max(0.0, (i - low) / max(high - low, 1e-3)))
                     freqs[i] *= 1.0 - slow + slow / factor
