@@ -74,3 +74,11 @@ def test_yarn_blends_between_its_two_pairs(dim, base, original, factor, ramp, mo
         assert f == pytest.approx(plain * kept + plain / factor * (1 - kept), rel=1e-13), i
         if plain * original > 2 * math.pi:  # more than one turn: not stretched all the way
             assert f > plain / factor * (1 + 1e-9)
+
+
+@pytest.mark.parametrize("betas", [{"beta_fast": 0}, {"beta_slow": 0.0}, {"beta_fast": -3}, {"beta_slow": float("nan")}, {"beta_fast": float("inf")},
+                                   {"beta_fast": 1, "beta_slow": 32}])
+def test_yarn_ramps_that_no_table_has(betas):
+    with pytest.raises(tq.TurqError) as e:
+        tq.RotaryTable.new(64, 16, scaling={"type": "yarn", "factor": 2.0, "original": 100, **betas})
+    assert e.value.status == 1

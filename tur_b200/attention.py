@@ -113,11 +113,15 @@ class RotaryTable:
                 if not 0.0 < n < math.inf:
                     raise TurqError(1, f"yarn scaling needs the original number of positions, got {scaling.get('original')}")
 
+                fast, slowest = float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
+                if not 0.0 < slowest <= fast < math.inf:
+                    raise TurqError(1, f"yarn scaling needs 0 < beta_slow <= beta_fast, got {slowest} and {fast}")
+
                 def pair_of(turns: float) -> float:
                     return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-                low = max(0, math.floor(pair_of(float(scaling.get("beta_fast", 32)))))
-                high = min(rotary_dim - 1, math.ceil(pair_of(float(scaling.get("beta_slow", 1)))))
+                low = max(0, math.floor(pair_of(fast)))
+                high = min(rotary_dim - 1, math.ceil(pair_of(slowest)))
                 for i in range(half):
                     slow = min(1.0, max(0.0, (i - low) / max(high - low, 1e-3)))
                     freqs[i] *= 1.0 - slow + slow / factor
