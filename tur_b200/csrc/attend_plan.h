@@ -77,6 +77,10 @@ inline TokenPlan plan_tokens(int64_t pairs, int64_t max_context, int sms, int ct
   return p;
 }
 
+// A warp's ring of copies: how many of its `own` steps have been requested once it has taken `taken` of them (the one that it takes next
+// among them). What it has not taken is still on its way.
+TQ_HD int ring_requested(int own, int taken, int stages) { return taken + stages < own ? taken + stages : own; }
+
 // ---- tiles of rows: TILE_ROWS rows (two row tiles of the tensor core) a CTA, a CTA an SM
 constexpr int TILE_ROWS = 256;
 constexpr int TILE_SPLITS = 32;     // pieces of a tile's keys that the join takes

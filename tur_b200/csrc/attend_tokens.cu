@@ -206,16 +206,12 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
     m[j][0] = m[j][1] = -INFINITY;
     l[j][0] = l[j][1] = 0.f;
   }
-  bool dead = false;
   const int r8 = lane & 7, mi = lane >> 3;
 
-  for (int step = warp, n = 0; step < steps; step += TOK_WARPS, n++) {
+  int step = warp, n = 0;  // n: steps taken
+  for (; step < steps; step += TOK_WARPS, n++) {
     const int stage = n % TOK_STAGES;
-    if (!dead && !bar_wait(&full[warp][stage], (n / TOK_STAGES) & 1, &abort_flag)) {
-      dead = true;
-      report(a.status, TURQ_E_TIMEOUT);
-    }
-    __syncwarp();
+    if (!__all_sync(0xFFFFFFFFu, bar_wait(&full[warp][stage], (n / TOK_STAGES) & 1, &abort_flag))) break;
     const uint32_t at = ring + stage * 2 * G::HALF, sc = ring + TOK_STAGES * 2 * G::HALF + stage * G::SCALES;
     const int k0 = step * KEYS;
 
@@ -374,6 +370,15 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // this stage was read, at a context's end also written, by ordinary accesses
     __syncwarp();
     if (lane == 0 && step + TOK_STAGES * TOK_WARPS < steps) issue(step + TOK_STAGES * TOK_WARPS, stage);
+  }
+  if (step < steps) {
+    // A wait ran out. Nothing more is requested; what has been lands before the ring is used for anything else and before the block ends.
+    report(a.status, TURQ_E_TIMEOUT);
+    const int own = (steps - warp + TOK_WARPS - 1) / TOK_WARPS;  // this warp's steps: warp, warp + TOK_WARPS, ...
+    for (int i = n; i < ring_requested(own, n, TOK_STAGES); i++) {
+      const long long t0 = clock64();
+      while (!bar_try(&full[warp][i % TOK_STAGES], (i / TOK_STAGES) & 1) && clock64() - t0 < TC_WAIT_CYCLES / 8) {}
+    }
   }
 
   // the four warps' results: each into its own ring, whose copies have all arrived
