@@ -336,8 +336,11 @@ int32_t turq_kv_read(turq_ctx* ctx, const turq_kv_cache* cache, const int64_t* d
  * One call takes single tokens, chunks and whole prompts together. A row that sees no key gives
  * zeros; rows outside every sequence are left as they were.
  * q is F16 or BF16, BF16 for a BF16 cache; out is F32, F16 or BF16, dense [n_tokens, n_q_heads,
- * head_dim], and may be q where type and stride agree. scale is positive, below 2^127. Products run on tensor cores in the cache's type (F16 for Q8_0) with sums, maxima
- * and outputs held in f32. Keys and values behind a context's end may hold anything; among those
+ * head_dim], and may be q where type and stride agree. scale is positive, below 2^127. Products run
+ * on tensor cores in the cache's type (F16 for Q8_0) with sums, maxima and outputs held in f32. A Q8_0
+ * block beyond F16, which is one with a scale above 515.5 (values beyond 65500), is infinite there: turq_kv_read
+ * returns it as it is, attention over a context that holds it gives what infinities give, and
+ * turq_ctx_poll_status reports it. Keys and values behind a context's end may hold anything; among those
  * of a context, values that a row does not see yet have to be finite.
  * max_new and max_context bound what the device arrays hold; what exceeds them, an id outside the
  * pages, or starts that descend are cut to the bounds (such a page reads as zeros) and

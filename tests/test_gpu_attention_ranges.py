@@ -1,4 +1,5 @@
-"""Attention over the cache where scores, keys and values leave the ordinary.
+"""Attention over the cache where scores, keys and values leave the ordinary: scores whose steps in f32 are large, NaN among the keys
+that a row sees, values of any size among those that it does not, blocks of Q8_0 beyond f16.
 
 Tolerances are those of the definition's roundings (a rounding to t is off by at most eps_t / 2 of the value): see each test."""
 import pytest
@@ -223,4 +224,39 @@ def test_every_border_of_a_long_context(kind, q_dtype, new, contexts, d):
             pair = held[seq][b - 1:b + 1, h]
             y = got[seq * new + r // group, h * group + r % group]
             assert ((y - pair.mean(0)).abs() <= rel * pair.abs().mean(0) + 2.0 ** -24).all(), (b, (y - pair.mean(0)).abs().max().item())
+    tq.context().poll_status()
+
+
+@pytest.mark.parametrize("q_dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_blocks_of_q8_0_up_to_what_f16_holds_and_beyond(q_dtype, d, new, which):
+    # 127 x 515.5 is the largest product of a quant and a scale that f16 holds (65468.5, rounded to 65472)
+    g = gen(47)
+    ctx = 150
+    cache, table = plain_cache("q8_0", ctx, d)
+    k, v = 0.01 * randn(g, ctx, 1, d), randn(g, ctx, 1, d)
+    big = 65400.0
+    (k if which == "k" else v)[70, 0, 5] = big
+    slots = torch.arange(ctx, device="cuda")
+    cache.write(k, v, slots)
+    kc, vc = cache.read(slots)
+    q = (0.001 * randn(g, new, 4, d)).to(q_dtype)
+    spans = [(new, ctx)]
+    check_attention(cache.attend(q, ints(0, new), ints(ctx), table, scale=1.0, out_dtype=torch.float32), q, kc, vc, spans, kind="q8_0", scale=1.0)
+    tq.context().poll_status()
+    (k if which == "k" else v)[70, 0, 5] = 66000.0
+    cache.write(k, v, slots)
+    tq.context().poll_status()  # the cache holds and returns it
+    kc, vc = cache.read(slots)
+    assert abs((kc if which == "k" else vc)[70, 0, 5].item() - 66000.0) <= 2.0 ** -8 * 66000
+    cache.attend(q, ints(0, new), ints(ctx), table, scale=1.0)
+    with pytest.raises(tq.TurqError) as e:
+        tq.context().poll_status()
+    assert e.value.status == 1
+    # behind a context's end it does not matter
+    short = 70
+    check_attention(cache.attend(q, ints(0, new), ints(short), table, scale=1.0, out_dtype=torch.float32), q, kc[:short], vc[:short], [(new, short)],
+                    kind="q8_0", scale=1.0)
     tq.context().poll_status()

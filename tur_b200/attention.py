@@ -288,7 +288,8 @@ class KvCache:
         starts[i] .. starts[i + 1] (int32 [n_seqs + 1]) of sequence i, whose context of contexts[i] tokens (int32 [n_seqs], the new
         ones last) lies in the pages page_table[i] (int32 [n_seqs, pages]). scale: 1 / sqrt(d) by default. `out` may be q. Single tokens,
         chunks and whole prompts go together; max_new and max_context are the longest of each that the call may meet (the
-        values on the device are not read here). `out` keeps its rows that belong to no sequence."""
+        values on the device are not read here). Q8_0 blocks of a context with scales above 515.5 (values beyond 65500, which f16 does
+        not hold) are infinities to the products, and context().poll_status() reports them. `out` keeps its rows that belong to no sequence."""
         dev, d = self._device, self.head_dim
         n, hq, qs = _rows(q, "q", dev, d)
         p_table = _vector(page_table, "page_table", dev, torch.int32, None)

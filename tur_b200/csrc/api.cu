@@ -260,7 +260,7 @@ int32_t turq_ctx_poll_status(turq_ctx* ctx, void* stream) {
     cudaMemsetAsync(ctx->gemv_ws, 0, turq::gemv_workspace_bytes(ctx->sm_count), s);
     cudaMemsetAsync(ctx->gemm_ws, 0, turq::gemm_workspace_bytes(ctx->sm_count), s);
     cudaStreamSynchronize(s);
-    if (st == TURQ_E_INVALID_ARG) return fail(ctx, st, "an id, position, slot, page or length on the device lies outside its table");
+    if (st == TURQ_E_INVALID_ARG) return fail(ctx, st, "an id, position, slot, page or length on the device lies outside its table, or attention met a Q8_0 block beyond f16");
     return fail(ctx, st, "a kernel gave up a bounded device-side wait (status %d)", st);
   }
   return TURQ_OK;

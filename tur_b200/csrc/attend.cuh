@@ -49,6 +49,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Q8_0 keys and values meet their products in f16: a block whose scale times 127 is beyond f16 (scales above 515.5) would be infinite
+// there. It is reported. What a thread has seen of scales' magnitudes, both of a pair; NaN passes through the products by itself.
+__device__ __forceinline__ void report_beyond_f16(const AttendArgs& a, __half2 largest) {
+  if (__hgt(__low2half(largest), __float2half_rn(515.5f)) || __hgt(__high2half(largest), __float2half_rn(515.5f)))
+    report(a.status, TURQ_E_INVALID_ARG);
+}
+
 // Scores are compared and subtracted as the products gave them, and multiplied (by scale x log2 e, times what a row of q was divided by)
 // afterwards: the product of a large score would be off by its own f32 rounding, in every weight a different one. Where pieces of a row meet,
 // their maxima come times the power of two in the row's multiplier, which is exact, and what is left of it, from 1 to 2, is the same for

@@ -689,6 +689,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       const int id0 = threadIdx.x - 320;
       int rs = 0, stage = 0;
       uint32_t rp = 0, ph = 0;
+      __half2 largest = __float2half2_rn(0.f);  // of the scales of keys and values of the context
       for (int j = 0; j < 2 * n_iter; j++) {
         const int keys = ctx - (begin + (j >> 1)) * TILE_N;  // that exist, of this tile
         tile_wait(&raw_full[rs], rp, abort_flag);
@@ -702,6 +703,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(src + id * 16));
           uint16_t sc;
           asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc) : "r"(src + TILE_N * D + (row * (D / 32) + (ch >> 1)) * 2));
+          if (row >= keys) sc = 0;  // anything may lie behind the context's end
           const __half2 scale = __half2half2(__ushort_as_half(sc)), off = __float2half2_rn(1152.f);
           const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
           uint32_t h[8];
@@ -710,10 +712,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
             h[2 * e] = h22u(__hmul2(__hsub2(pair01(x[e]), off), scale));
             h[2 * e + 1] = h22u(__hmul2(__hsub2(pair23(x[e]), off), scale));
           }
-          if (row >= keys) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) h[e] = 0u;
-          }
+          largest = __hmax2(largest, __habs2(scale));
           const uint32_t to = dst + (ch >> 2) * HB + row * 128;
           const int c0 = ((2 * ch) & 7) ^ (row & 7), c1 = ((2 * ch + 1) & 7) ^ (row & 7);
           asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + (c0 << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
@@ -728,6 +727,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
         if (++rs == G::RAW_STAGES) { rs = 0; rp ^= 1u; }
         if (++stage == ST) { stage = 0; ph ^= 1u; }
       }
+      report_beyond_f16(a, largest);
     }
   }
   tc_before();

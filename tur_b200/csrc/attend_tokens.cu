@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
     l[j][0] = l[j][1] = 0.f;
   }
   const int r8 = lane & 7, mi = lane >> 3;
+  __half2 largest = __float2half2_rn(0.f);  // of the scales of keys and values of the context
 
   int step = warp, n = 0;  // n: steps taken
   for (; step < steps; step += TOK_WARPS, n++) {
@@ -214,6 +215,19 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
     if (!__all_sync(0xFFFFFFFFu, bar_wait(&full[warp][stage], (n / TOK_STAGES) & 1, &abort_flag))) break;
     const uint32_t at = ring + stage * 2 * G::HALF, sc = ring + TOK_STAGES * 2 * G::HALF + stage * G::SCALES;
     const int k0 = step * KEYS;
+    if (Q8) {  // a key's scales (lanes 0 to 15) or a value's each: those behind the context's end are anything
+#pragma unroll
+      for (int kt = 0; kt < KT; kt++) {
+        uint32_t w[D / 64];
+        const uint32_t from = sc + ((lane >> 4) * KT + kt) * G::SC_AT + (lane & 15) * (D / 16);
+        if (k0 + 16 * kt + (lane & 15) < keys) {
+          if (D == 128) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[D / 64 - 1]) : "r"(from));
+          else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(from));
+#pragma unroll
+          for (int i = 0; i < D / 64; i++) largest = __hmax2(largest, __habs2(u2h2(w[i])));
+        }
+      }
+    }
 
     // S^T: lane (g, c) gets keys g and g + 8 of a tile for rows 2c, 2c + 1
     float s[KT][NR][4];
@@ -380,6 +394,8 @@ __global__ void __launch_bounds__(32 * TOK_WARPS, TokGeom<D, Q8, NR>::CTAS) atte
       while (!bar_try(&full[warp][i % TOK_STAGES], (i / TOK_STAGES) & 1) && clock64() - t0 < TC_WAIT_CYCLES / 8) {}
     }
   }
+
+  if (Q8) report_beyond_f16(a, largest);
 
   // the four warps' results: each into its own ring, whose copies have all arrived
   __syncwarp();
