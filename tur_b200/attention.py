@@ -289,7 +289,8 @@ class KvCache:
         ones last) lies in the pages page_table[i] (int32 [n_seqs, pages]). scale: 1 / sqrt(d) by default. `out` may be q. Single tokens,
         chunks and whole prompts go together; max_new and max_context are the longest of each that the call may meet (the
         values on the device are not read here). Q8_0 blocks of a context with scales above 515.5 (values beyond 65500, which f16 does
-        not hold) are infinities to the products, and context().poll_status() reports them. `out` keeps its rows that belong to no sequence."""
+        not hold) are infinities to the products, and context().poll_status() reports them. `out` keeps its rows that belong to no sequence; without `out` they hold
+        anything."""
         dev, d = self._device, self.head_dim
         n, hq, qs = _rows(q, "q", dev, d)
         p_table = _vector(page_table, "page_table", dev, torch.int32, None)
@@ -343,12 +344,14 @@ class Attention:
                 contexts: torch.Tensor, page_table: torch.Tensor, *, max_new: Optional[int] = None, max_context: Optional[int] = None,
                 mode: Mode = Mode.AUTO) -> torch.Tensor:
         """x [n_tokens, hidden] (f32 or bf16), the packed new tokens of all sequences -> [n_tokens, hidden] f32. The other
-        arguments are those of KvCache.append and KvCache.attend."""
+        arguments are those of KvCache.append and KvCache.attend. Rows of tokens that belong to no sequence (the padding of a
+        captured batch) follow from x alone and mean nothing."""
         linears = (self.q, self.k, self.v)
         biases = [l.bias for l in linears] if any(l.bias is not None for l in linears) else None
         q, k, v = QMatMul.forward_multi([l.qmatmul for l in linears], x, biases=biases, mode=mode)
         q = cache.append(q, k, v, positions, table, slots, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.eps)
-        y = cache.attend(q, starts, contexts, page_table, max_new=max_new, max_context=max_context, scale=self.scale)
+        # into q's own memory: rows of tokens of no sequence then hold their queries, and not what the memory held before
+        y = cache.attend(q, starts, contexts, page_table, max_new=max_new, max_context=max_context, scale=self.scale, out=q)
         return self.o.forward(y.view(y.shape[0], -1), mode=mode)
 
     __call__ = forward
