@@ -322,15 +322,21 @@ class KvCache:
 
 class Attention:
     """tur's attention block on a quantized layer (Qwen3Attention, src/models/qwen3.rs:205-222, 263-505; Granite's without
-    head norms): attn_q|k|v in one call, norms, rotation and cache write in one pass, attention, attn_output."""
+    head norms): attn_q|k|v in one call, norms, rotation and cache write in one pass, attention, attn_output. q_dtype: the type of the
+    queries between them, bfloat16 by default; float16 for F16 and Q8_0 caches keeps three bits more of queries below 65504. What
+    goes to attn_output is bfloat16, with float16 queries or mode EXACT_F32 float32."""
 
     def __init__(self, q: LinearX, k: LinearX, v: LinearX, o: LinearX, head_dim: int, q_norm: Optional[torch.Tensor] = None,
-                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, scale: Optional[float] = None):
+                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, scale: Optional[float] = None,
+                 q_dtype: torch.dtype = torch.bfloat16):
+        if q_dtype not in (torch.bfloat16, torch.float16):
+            raise TurqError(3, f"q_dtype {q_dtype} is neither bfloat16 nor float16")
         self.q, self.k, self.v, self.o = q, k, v, o
-        self.head_dim, self.q_norm, self.k_norm, self.eps, self.scale = head_dim, q_norm, k_norm, eps, scale
+        self.head_dim, self.q_norm, self.k_norm, self.eps, self.scale, self.q_dtype = head_dim, q_norm, k_norm, eps, scale, q_dtype
 
     @classmethod
-    def new(cls, vb, hidden: int, n_heads: int, n_kv_heads: int, head_dim: int, eps: float = 1e-6, scale: Optional[float] = None) -> "Attention":
+    def new(cls, vb, hidden: int, n_heads: int, n_kv_heads: int, head_dim: int, eps: float = 1e-6, scale: Optional[float] = None,
+            q_dtype: torch.dtype = torch.bfloat16) -> "Attention":
         """From the tensors of one block (`vb.pp("blk").pp(i)`): attn_q, attn_k, attn_v, attn_output, and attn_q_norm /
         attn_k_norm where the file has them."""
         def norm(name):
@@ -338,7 +344,7 @@ class Attention:
 
         return cls(linear(hidden, n_heads * head_dim, vb.pp("attn_q")), linear(hidden, n_kv_heads * head_dim, vb.pp("attn_k")),
                    linear(hidden, n_kv_heads * head_dim, vb.pp("attn_v")), linear(n_heads * head_dim, hidden, vb.pp("attn_output")),
-                   head_dim, norm("attn_q_norm"), norm("attn_k_norm"), eps, scale)
+                   head_dim, norm("attn_q_norm"), norm("attn_k_norm"), eps, scale, q_dtype)
 
     def forward(self, x: torch.Tensor, cache: KvCache, table: RotaryTable, positions: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor,
                 contexts: torch.Tensor, page_table: torch.Tensor, *, max_new: Optional[int] = None, max_context: Optional[int] = None,
@@ -349,9 +355,12 @@ class Attention:
         linears = (self.q, self.k, self.v)
         biases = [l.bias for l in linears] if any(l.bias is not None for l in linears) else None
         q, k, v = QMatMul.forward_multi([l.qmatmul for l in linears], x, biases=biases, mode=mode)
-        q = cache.append(q, k, v, positions, table, slots, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.eps)
-        # into q's own memory: rows of tokens of no sequence then hold their queries, and not what the memory held before
-        y = cache.attend(q, starts, contexts, page_table, max_new=max_new, max_context=max_context, scale=self.scale, out=q)
+        q = cache.append(q, k, v, positions, table, slots, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.eps, out_dtype=self.q_dtype)
+        # Into q's own memory, or into zeros: rows of tokens of no sequence hold their queries then, and not what the memory held before.
+        # f32 where its bits are asked for: it costs 2 us a call, and twice the bytes (2048 tokens 5 % of a layer's time).
+        wide = mode == Mode.EXACT_F32 or q.dtype is not torch.bfloat16
+        y = cache.attend(q, starts, contexts, page_table, max_new=max_new, max_context=max_context, scale=self.scale,
+                         out=torch.zeros_like(q, dtype=torch.float32) if wide else q)
         return self.o.forward(y.view(y.shape[0], -1), mode=mode)
 
     __call__ = forward
