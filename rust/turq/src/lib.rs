@@ -454,6 +454,72 @@ pub struct Rotary {
     pub interleaved: bool,
 }
 
+/// Fills `dev_table` with cos and sin of position * `freqs[i]` times `scale`, `[n_positions, freqs.len(), 2]` f32 (`src/models/qwen3.rs:64-78`).
+///
+/// # Safety
+/// `dev_table` must be a device pointer on the context's device with that many elements, 16-byte aligned, and stay valid until the
+/// stream has run the work.
+pub unsafe fn rope_table(ctx: &Context, freqs: &[f64], n_positions: i64, scale: f64, dev_table: *mut f32, stream: *mut c_void) -> Result<()> {
+    // SAFETY: freqs are live and read before the call returns; forwarded contract of this function.
+    let st = unsafe { sys::turq_rope_table(ctx.h, freqs.as_ptr(), freqs.len() as i32, n_positions, scale, dev_table, stream) };
+    ctx.check(st)
+}
+
+/// RMSNorm of every head (where a weight is given) and rotation of q and k (`src/models/qwen3.rs:277-290`) into dense tensors.
+///
+/// # Safety
+/// The pointers must be device pointers on the context's device with the sizes `turq_qk_norm_rope` states, and stay valid until the
+/// stream has run the work.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn qk_norm_rope(
+    ctx: &Context,
+    q: HeadRows,
+    k: HeadRows,
+    x_dtype: GgmlDType,
+    n: usize,
+    n_heads: usize,
+    n_kv_heads: usize,
+    head_dim: usize,
+    dev_q_weight: *const f32,
+    dev_k_weight: *const f32,
+    eps: f32,
+    rotary: &Rotary,
+    dev_positions: *const i32,
+    out_dtype: GgmlDType,
+    dev_q_out: *mut c_void,
+    dev_k_out: *mut c_void,
+    stream: *mut c_void,
+) -> Result<()> {
+    // SAFETY: forwarded contract of this function.
+    let st = unsafe {
+        sys::turq_qk_norm_rope(
+            ctx.h,
+            q.dev,
+            q.stride,
+            k.dev,
+            k.stride,
+            x_dtype as i32,
+            n as i64,
+            n_heads as i32,
+            n_kv_heads as i32,
+            head_dim as i32,
+            dev_q_weight,
+            dev_k_weight,
+            eps,
+            rotary.dev_table,
+            rotary.n_positions,
+            rotary.rotary_dim,
+            i32::from(rotary.interleaved),
+            dev_positions,
+            out_dtype as i32,
+            dev_q_out,
+            dev_k_out,
+            stream,
+        )
+    };
+    ctx.check(st)
+}
+
 /// The new tokens of several sequences over their pages (`turq_kv_attention`).
 #[derive(Debug, Clone, Copy)]
 pub struct Batch {
@@ -550,6 +616,28 @@ impl KvCache {
                 stream,
             )
         };
+        self.ctx.check(st)
+    }
+
+    /// Keys and values as they are into their slots, rounded to the cache's type or quantized.
+    ///
+    /// # Safety
+    /// As for `append`, with the sizes `turq_kv_write` states.
+    pub unsafe fn write(&self, k: HeadRows, v: HeadRows, x_dtype: GgmlDType, n: usize, dev_slots: *const i64, stream: *mut c_void) -> Result<()> {
+        // SAFETY: forwarded contract of this function.
+        let st = unsafe {
+            sys::turq_kv_write(self.ctx.h, self.h, k.dev, k.stride, v.dev, v.stride, x_dtype as i32, n as i64, dev_slots, stream)
+        };
+        self.ctx.check(st)
+    }
+
+    /// Keys and values of the slots into dense `[n, n_kv_heads, head_dim]` tensors.
+    ///
+    /// # Safety
+    /// As for `append`, with the sizes `turq_kv_read` states.
+    pub unsafe fn read(&self, dev_slots: *const i64, n: usize, out_dtype: GgmlDType, dev_k: *mut c_void, dev_v: *mut c_void, stream: *mut c_void) -> Result<()> {
+        // SAFETY: forwarded contract of this function.
+        let st = unsafe { sys::turq_kv_read(self.ctx.h, self.h, dev_slots, n as i64, out_dtype as i32, dev_k, dev_v, stream) };
         self.ctx.check(st)
     }
 

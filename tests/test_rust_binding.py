@@ -57,3 +57,20 @@ def test_safe_wrapper_only_calls_declared_functions_and_never_panics():
     for banned in (".unwrap()", ".expect(", "panic!(", "unreachable!(", "todo!(", "unimplemented!("):
         assert banned not in code, f"the wrapper must not use {banned} (the reference denies it: Cargo.toml:79-86)"
     assert "impl Drop for QTensor" in code and "#[derive(Clone)]\npub struct QMatMul" in src
+
+
+def test_safe_wrapper_reaches_every_entry_of_the_cache_and_the_rotation():
+    """With as many arguments, in the extern block's order where they carry its names."""
+    gen = _gen()
+    src = re.sub(r"//.*", "", open(os.path.join(ROOT, "rust", "turq", "src", "lib.rs")).read())
+    for name, _, args in gen.parse_rust():
+        if not name.startswith(("turq_kv_", "turq_rope_", "turq_qk_")) or name in ("turq_kv_cache_bytes", "turq_kv_cache_layout"):  # the library's own memory
+            continue
+        call = re.search(rf"sys::{name}\(((?:[^()]|\([^()]*\))*)\)", src)
+        assert call, f"the wrapper does not call {name}"
+        given = [a.strip() for a in re.split(r",(?![^()]*\))", call.group(1)) if a.strip()]
+        assert len(given) == len(args), (name, given)
+        names = [a[0] if isinstance(a, tuple) else a.split(":")[0].strip() for a in args]
+        for want, got in zip(names, given):
+            if re.fullmatch(r"(dev|host)_\w+", got):
+                assert want.startswith(got), (name, want, got)
