@@ -28,10 +28,7 @@ static AttendWorkspace attend_workspace(const turq_kv_cache* kc, int64_t n_token
   w.tiles = most * group > TOKEN_ROWS;
   if (w.tokens) {
     w.part_rows = (int)(w.tiles ? TOKEN_ROWS : most * group);
-    // Beside tiles the tokens get the SMs that those leave, late: chunks for half as many sequences, shorter and more, end sooner (six
-    // sequences, 512 + 33 new tokens and four that decode: 98 us, so 86).
-    const int64_t pairs = (int64_t)n_seqs * kc->n_kv_heads;
-    const TokenPlan p = plan_tokens(w.tiles ? (pairs + 1) / 2 : pairs, max_context, kc->sm_count, token_ctas(kc->dtype == TURQ_Q8_0, w.part_rows <= 8));
+    const TokenPlan p = plan_tokens((int64_t)n_seqs * kc->n_kv_heads, max_context, kc->sm_count, token_ctas(kc->dtype == TURQ_Q8_0, w.part_rows <= 8), w.tiles);
     w.chunk = (int)p.chunk;
     w.max_chunks = (int)p.chunks;
     w.cluster = p.cluster;

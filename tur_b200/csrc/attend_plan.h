@@ -66,11 +66,17 @@ inline int64_t plan_token_chunk(int64_t pairs /* sequences x key heads */, int64
 // against launch: 1024 keys 6.2 / - against 6.6 / -, 4096 keys 9.2 / 11.0 against 8.2 / 16.1 (the second launch and the workspace cost
 // the host 5); 8192 keys in chunks of 512 12.3 against 9.9, which is why a chunk may not be longer than 256 for it.
 constexpr int TOKEN_CLUSTER = 16, TOKEN_CLUSTER_KEYS = 256;
+// Beside tiles the tokens get the SMs that those leave, late: chunks for half as many pairs, which are shorter and more, end sooner, while
+// whether clusters find room goes by the pairs that there are. us, a chunk of 512 on 4096 keys and so many users at 200 to 6000 (32
+// heads on 8 of 128), length by half of the pairs / by all, bf16 and Q8_0: 4 users 62.1 / 63.1 and 66.0 / 67.1, 8 73.5 / 74.7 and 76.7 /
+// 84.7, 16 87.3 / 90.9 and 89.3 / 108.4, 32 142.0 / 130.8 and 112.9 / 114.2, 64 205.7 / 205.3 and 177.0 / 175.9; six sequences
+// (512 of 8000, 33 of 1000, four users; 40 on 10 of 64, f16) 86.1 / 95.9. Room by half of the pairs too: 8 80.2 and 76.7, 16 95.0 and
+// 110.4, 32 136.0 and 134.3.
 struct TokenPlan { int64_t chunk, chunks; bool cluster; };
-inline TokenPlan plan_tokens(int64_t pairs, int64_t max_context, int sms, int ctas) {
+inline TokenPlan plan_tokens(int64_t pairs, int64_t max_context, int sms, int ctas, bool beside = false) {
   TokenPlan p;
   const int64_t sixteenth = (max_context + TOKEN_CLUSTER * TOKEN_STEP - 1) / (TOKEN_CLUSTER * TOKEN_STEP) * TOKEN_STEP;
-  p.chunk = plan_token_chunk(pairs, max_context, sms, ctas);
+  p.chunk = plan_token_chunk(beside ? (pairs + 1) / 2 : pairs, max_context, sms, ctas);
   if (sixteenth > p.chunk && sixteenth <= TOKEN_CLUSTER_KEYS && pairs * TOKEN_CLUSTER <= sms) p.chunk = sixteenth;
   p.chunks = max_context <= p.chunk ? 1 : (max_context + p.chunk - 1) / p.chunk;
   p.cluster = p.chunks > 1 && p.chunks <= TOKEN_CLUSTER && pairs * p.chunks <= (int64_t)(p.chunks <= 8 ? ctas : 1) * sms;
