@@ -260,3 +260,19 @@ def test_blocks_of_q8_0_up_to_what_f16_holds_and_beyond(q_dtype, d, new, which):
     check_attention(cache.attend(q, ints(0, new), ints(short), table, scale=1.0, out_dtype=torch.float32), q, kc[:short], vc[:short], [(new, short)],
                     kind="q8_0", scale=1.0)
     tq.context().poll_status()
+
+
+@pytest.mark.parametrize("kind,q_dtype", TYPES)
+@pytest.mark.parametrize("d,group", [(128, 128), (128, 3), (64, 64), (64, 17)])
+def test_many_rows_that_see_no_key(kind, q_dtype, d, group):
+    # Tiles without a key, by hundreds, on the SMs beside tiles with some and behind one another: zeros, exactly, whatever the queries are.
+    spans = [(1 + i % 9 * (40 // group + 1), 0) for i in range(60)] + [(300, 300)] + [(20 + i, 0) for i in range(60)]
+    cache, table, q, starts, contexts, k, v = make_case(49, spans, kind, q_dtype, 2 * group, 2, d, 16)
+    full = slice(int(starts[60]), int(starts[61]))
+    out = torch.empty_like(q)
+    for _ in range(30):
+        out.fill_(7.0)
+        cache.attend(q, starts, contexts, table, out=out)
+        assert not out[:full.start].any() and not out[full.stop:].any()
+    check_attention(out[full], q[full], k, v, [(300, 300)], kind=kind)
+    tq.context().poll_status()

@@ -306,8 +306,9 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
     row_at[t][r] = live ? rt | (r - rt * a.group) << 8 : -1;  // once, and not for every 16 bytes that come or go
     tile_sync(1 + t);
     // Q into the operand layout, D / 8 lanes a row (a row a thread, every load would touch 32 lines: 7300 cycles against 3500); on f16
-    // caches a bf16 row by the power of two that its largest element fits.
-    if (t < tiles) {
+    // caches a bf16 row by the power of two that its largest element fits. Not where there is no key: the result goes out through the same
+    // memory, and nothing between the two would wait for the last thread to have brought its part of Q.
+    if (t < tiles && n_iter > 0) {
       constexpr int L = D / 8, ROWS = TILE_M / L;  // rows of a pass
       const int ch = r % L;
       const uint16_t* const qp = a.q + (sp.first + work.tok0 + t * tpt) * a.q_stride + (int64_t)head * a.group * D + 8 * ch;
@@ -342,7 +343,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
       if (lane == 0) bar_arrive(&q_full[t]);
       if (convert) tile_sync(1 + t);
     }
-    const float mul = !BF && a.q_bf16 && t < tiles ? row_mul(a, row_up[t][r]) : a.scale_log2;
+    const float mul = !BF && a.q_bf16 && t < tiles && n_iter > 0 ? row_mul(a, row_up[t][r]) : a.scale_log2;
     const int seen = live ? (int)min(sp.ctx, keys_seen(sp, tok, a.causal)) : INT32_MAX;  // rows that do not exist ask for no mask
     // keys that every row of the warp sees
     int least = seen;
