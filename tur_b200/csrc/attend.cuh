@@ -4,6 +4,7 @@
 #include "attend_plan.h"
 #include "device_utils.cuh"
 #include "kvcache.cuh"
+#include "tc_common.cuh"
 
 namespace turq {
 
@@ -67,6 +68,29 @@ __device__ __forceinline__ float joined_max(float m, float mul) {
   return m == -INFINITY ? m : m * __uint_as_float(__float_as_uint(mul) & 0x7F800000u);
 }
 __device__ __forceinline__ float joined_factor(const AttendArgs& a) { return __uint_as_float((__float_as_uint(a.scale_log2) & 0x7FFFFFu) | 0x3F800000u); }
+
+// Two f32 rounded to the 16-bit type of the products.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if (BF) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+  const __half2 t = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+// Four int8 -> half2 pairs (b0, b1), (b2, b3), exact before the scale: 1024 + (q + 128) less 1152.
+__device__ __forceinline__ void halves_of(uint32_t w, __half2 scale, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  const __half2 off = __float2half2_rn(1152.f);
+  lo = h22u(__hmul2(__hsub2(pair01(u), off), scale));
+  hi = h22u(__hmul2(__hsub2(pair23(u), off), scale));
+}
+// A box of a plane of pages to shared memory, reported to a barrier there.
+__device__ __forceinline__ void copy_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
 
 // Two neighbouring elements of the output, rounded once.
 __device__ __forceinline__ void store_out2(void* out, int dtype, int64_t i, float a, float b) {

@@ -75,10 +75,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db),
                "r"(idesc), "r"(acc) : "memory");
 }
-__device__ __forceinline__ void tile_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
 // The largest of three, one instruction.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -127,15 +123,6 @@ __device__ __forceinline__ void ex2_pair(uint64_t v, float& x, float& y) {
   float tx, ty;
   un2(t, tx, ty);
   un2(mul2(p, f2(__int_as_float(__float_as_int(tx) << 23), __int_as_float(__float_as_int(ty) << 23))), x, y);
-}
-template <bool BF>
-__device__ __forceinline__ uint32_t pack_p(float a, float b) {
-  if (BF) {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
-  }
-  const __half2 t = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&t);
 }
 
 // Bounded: after an expiry the abort flag ends every further wait, and what a loop then does stays within its buffers.
@@ -333,7 +320,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
           if (ch == 0) row_up[t][row] = __uint_as_float((uint32_t)(127 + e2) << 23);
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = pack_p<false>(__uint_as_float(x[e] << 16) * down, __uint_as_float(x[e] & 0xFFFF0000u) * down);
+          for (int e = 0; e < 4; e++) x[e] = pack16<false>(__uint_as_float(x[e] << 16) * down, __uint_as_float(x[e] & 0xFFFF0000u) * down);
         }
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(sQ + t * OP + (ch >> 3) * HB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)), "r"(w[i].x),
                      "r"(w[i].y), "r"(w[i].z), "r"(w[i].w) : "memory");
@@ -449,7 +436,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
               y = ex2(y);
             }
             sum[i & 1] = add2(sum[i & 1], f2(x, y));
-            p[i] = pack_p<BF>(x, y);
+            p[i] = pack16<BF>(x, y);
           }
           tmem_st16(tP + 16 * h, p);
           if (h % 2 == 1) {  // half of the weights: their product may start
@@ -526,7 +513,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           for (int e = 0; e < 32; e += 8) {
             uint32_t w[4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) w[q] = bf ? pack_p<true>(o[e + 2 * q], o[e + 2 * q + 1]) : pack_p<false>(o[e + 2 * q], o[e + 2 * q + 1]);
+            for (int q = 0; q < 4; q++) w[q] = bf ? pack16<true>(o[e + 2 * q], o[e + 2 * q + 1]) : pack16<false>(o[e + 2 * q], o[e + 2 * q + 1]);
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + r * 2 * D + (((4 * i + e / 8) ^ (r & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                          "r"(w[3]) : "memory");
           }
@@ -644,7 +631,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
             __syncwarp();
             if (z >= 0) {
 #pragma unroll
-              for (int h = 0; h < G::HALVES; h++) tile_box3(at + h * HB, kv ? &maps.v : &maps.k, 64 * h, y, z, bar);
+              for (int h = 0; h < G::HALVES; h++) copy_box3(at + h * HB, kv ? &maps.v : &maps.k, 64 * h, y, z, bar);
             }
             if (++stage == ST) { stage = 0; ph ^= 1u; }
           } else {
@@ -652,7 +639,7 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
             const uint32_t bar = s_u32(&raw_full[stage]), at = sRaw + stage * G::RAW;
             if (lane == 0) bar_expect_tx(&raw_full[stage], n * box * D);
             __syncwarp();
-            if (z >= 0) tile_box3(at + lane * box * D, kv ? &maps.v : &maps.k, 0, y, z, bar);
+            if (z >= 0) copy_box3(at + lane * box * D, kv ? &maps.v : &maps.k, 0, y, z, bar);
             // Scales are too small for boxes (16 of 64 bytes a tile; with pages of 16 tokens head dimension 64 then waits for the copies' rate:
             // one prompt of 8192 tokens 618 us, 541 this way): 16 bytes at a time, zeros where there is no page.
             const __half* const from = kv ? a.cache.vs : a.cache.ks;
@@ -705,14 +692,12 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
           uint16_t sc;
           asm volatile("ld.shared.u16 %0, [%1];" : "=h"(sc) : "r"(src + TILE_N * D + (row * (D / 32) + (ch >> 1)) * 2));
           if (row >= keys) sc = 0;  // anything may lie behind the context's end
-          const __half2 scale = __half2half2(__ushort_as_half(sc)), off = __float2half2_rn(1152.f);
-          const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+          const __half2 scale = __half2half2(__ushort_as_half(sc));
           uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            h[2 * e] = h22u(__hmul2(__hsub2(pair01(x[e]), off), scale));
-            h[2 * e + 1] = h22u(__hmul2(__hsub2(pair23(x[e]), off), scale));
-          }
+          halves_of(w.x, scale, h[0], h[1]);
+          halves_of(w.y, scale, h[2], h[3]);
+          halves_of(w.z, scale, h[4], h[5]);
+          halves_of(w.w, scale, h[6], h[7]);
           largest = __hmax2(largest, __habs2(scale));
           const uint32_t to = dst + (ch >> 2) * HB + row * 128;
           const int c0 = ((2 * ch) & 7) ^ (row & 7), c1 = ((2 * ch + 1) & 7) ^ (row & 7);

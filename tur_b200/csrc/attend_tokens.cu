@@ -58,27 +58,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <bool BF>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-  if (BF) {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
-  }
-  const __half2 t = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&t);
-}
-// Four int8 -> half2 pairs (b0, b1), (b2, b3), exact: 1024 + (q + 128) less 1152.
-__device__ __forceinline__ void halves_of(uint32_t w, __half2 scale, uint32_t& lo, uint32_t& hi) {
-  const uint32_t u = w ^ 0x80808080u;
-  const __half2 off = __float2half2_rn(1152.f);
-  lo = h22u(__hmul2(__hsub2(pair01(u), off), scale));
-  hi = h22u(__hmul2(__hsub2(pair23(u), off), scale));
-}
-
-__device__ __forceinline__ void copy_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
 __device__ __forceinline__ void copy_box2(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
