@@ -107,8 +107,10 @@ int32_t turq_ctx_reserve(turq_ctx* ctx, int64_t max_m, int64_t max_k, int64_t ma
  * falls back to INT8_ACT for in-features that are not a multiple of 64). */
 int32_t turq_ctx_set_auto_policy(turq_ctx* ctx, int32_t mode);
 /* Kernels never trap: a device-side wait that runs out (mbarrier, cross-CTA hand-over) stops
- * the kernel and records a status word. This call synchronizes `stream`, returns TURQ_OK or
- * the recorded status (TURQ_E_TIMEOUT) and clears it. */
+ * the kernel and records a status word (TURQ_E_TIMEOUT). So does a kernel that meets data on the
+ * device which its entry cannot check (TURQ_E_INVALID_ARG: an id, position, slot, page or length outside
+ * its table, a Q8_0 block beyond what attention takes). This call synchronizes `stream`, returns
+ * TURQ_OK or the recorded status and clears it. */
 int32_t turq_ctx_poll_status(turq_ctx* ctx, void* stream);
 /* Number of kernels this context has launched so far (bookkeeping for benchmarks). */
 int64_t turq_ctx_launch_count(const turq_ctx* ctx);
@@ -313,7 +315,8 @@ int32_t turq_kv_cache_layout(const turq_kv_cache* cache, void** dev_memory, int6
  * pass, rounded once or quantized: d = amax / 127 per 32 elements in f32, stored as f16, value =
  * round-half-away(x * (1 / d)). dev_slots are int64, one per token: a negative one leaves the
  * cache alone (padding), one past the last page too and turq_ctx_poll_status reports it. Two
- * tokens of a call must not name one slot: what it then holds is either's, element by element. */
+ * tokens of a call must not name one slot: what it then holds is either's, store by store (a Q8_0
+ * block may get the quants of one and the scale of the other). */
 int32_t turq_kv_append(turq_ctx* ctx, turq_kv_cache* cache, const void* dev_q, int64_t q_stride, const void* dev_k, int64_t k_stride,
                        const void* dev_v, int64_t v_stride, int32_t x_dtype, int64_t n_tokens, int32_t n_q_heads,
                        const float* dev_q_weight, const float* dev_k_weight, float eps, const float* dev_table, int64_t n_positions,

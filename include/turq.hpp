@@ -62,7 +62,7 @@ class Context {
   void check(int32_t st) const {
     if (st != TURQ_OK) throw Error(st, turq_last_error(h_));
   }
-  // Synchronizes `stream` and throws if a kernel gave up a bounded device-side wait.
+  // Synchronizes `stream` and throws if a kernel gave up a bounded device-side wait or met an id, slot or length outside its table.
   void poll_status(void* stream = nullptr) const { check(turq_ctx_poll_status(h_, stream)); }
   // Sizes the scratch for the largest call so that no later call allocates.
   void reserve(int64_t max_m, int64_t max_k, int64_t max_n) const { check(turq_ctx_reserve(h_, max_m, max_k, max_n)); }

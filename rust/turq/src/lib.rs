@@ -149,7 +149,7 @@ impl Context {
         self.check(unsafe { sys::turq_ctx_set_auto_policy(self.h, mode as i32) })
     }
 
-    /// Synchronizes `stream` and reports a kernel that gave up a bounded device-side wait.
+    /// Synchronizes `stream` and reports a kernel that gave up a bounded device-side wait, or met an id, slot or length outside its table.
     pub fn poll_status(&self, stream: *mut c_void) -> Result<()> {
         // SAFETY: live context; `stream` is a cudaStream_t or null.
         self.check(unsafe { sys::turq_ctx_poll_status(self.h, stream) })

@@ -92,6 +92,11 @@ constexpr int TILE_ROWS = 256;
 constexpr int TILE_SPLITS = 32;     // pieces of a tile's keys that the join takes
 constexpr int TILE_OVERHEAD = 4;    // what a CTA costs beside its key tiles, and what the join does, in key tiles of 128
 constexpr int TILE_WAVES = 3;       // pieces are no more than that many CTAs an SM
+// Both measured, us (least of four medians; 32 heads on 8 of 128, bf16, but where 40 on 10 of 64, f16). Overhead 2 / 4 / 8: 128 new tokens on
+// 20000 keys 59.0 / 59.0 / 59.0, 512 on 8000 74.5 / 74.5 / 74.6, 4 x 200 on 6000 95.5 / 95.4 / 95.5, 512 on 8000 (of 64) 88.5 / 82.4 / 84.5, with
+// 33 on 1000 beside it 85.1 / 83.4 / 84.3. Waves 2 / 3 / 4: 128 on 20000 63.3 / 59.0 / 59.2, 512 on 8000 75.9 / 74.5 / 76.0, 1500 on 30000
+// 790 / 647 / 606, 300 on 4000 40.4 / 40.2 / 38.8, 4 x 200 on 6000 95.7 / 95.4 / 96.9, 512 on 8000 (of 64) 83.3 / 82.4 / 83.5, 3 x 1000 on their
+// own 46.9 / 46.9 / 46.8: 3 is the middle of what small and large calls would take.
 // What cutting the keys of each of `ctas` tiles (the longest with `iters` key tiles) into s pieces costs: waves x (key tiles + overhead).
 // The kernel takes the s that costs least.
 TQ_HD int64_t tile_split_cost(int s, int ctas, int iters, int pieces, int sms) {

@@ -399,7 +399,8 @@ attend_tiles_kernel(const __grid_constant__ TileMaps maps, const __grid_constant
             tmem_wait_st();
           }
           // A weight's exponent is one FMA, s x mul - sub: off by what m x mul loses in rounding, the same for all weights until m changes. From
-          // 2^10 on that is 2^-14 and more: such rows (above = m says so) subtract m from their scores before they multiply.
+          // 2^10 on that is 2^-14 and more: such rows (above = m says so) subtract m from their scores before they multiply. Where all rows
+          // do, a prompt of 4096 tokens takes a fifth longer (132 us, so 160; head dimension 64 135 and 162), where none does as long.
           sub = m == -INFINITY ? 0.f : m * mul;
           above = m + 8.f / mul;
           if (fabsf(sub) > 1024.f) {

@@ -73,7 +73,8 @@ class _Context:
             raise TurqError(st, _lib.load().turq_last_error(self.handle).decode())
 
     def poll_status(self) -> None:
-        """Synchronizes the current stream and raises if a kernel gave up a bounded wait."""
+        """Synchronizes the current stream and raises if a kernel gave up a bounded wait, or met an id, position, slot, page or length
+        outside its table."""
         self.check(_lib.load().turq_ctx_poll_status(self.handle, _stream_ptr(self.device)))
 
     def launch_count(self) -> int:
