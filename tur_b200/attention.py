@@ -288,11 +288,12 @@ class KvCache:
         starts[i] .. starts[i + 1] (int32 [n_seqs + 1]) of sequence i, whose context of contexts[i] tokens (int32 [n_seqs], the new
         ones last) lies in the pages page_table[i] (int32 [n_seqs, pages]). scale: 1 / sqrt(d) by default. `out` may be q. Single tokens,
         chunks and whole prompts go together; max_new and max_context are the longest of each that the call may meet (the
-        values on the device are not read here), by default all tokens and the whole page table. How the work is cut goes by them, so
-        they are worth giving, and as small as they are: 64 users of one token each take 154 us without max_new=1 and 115 with it (Q8_0,
-        contexts to 8000), one user at 4096 keys 34 us with max_context=131072 and 8.6 with 4096. Q8_0 blocks of a context with scales above 515.5 (values beyond 65500, which f16 does
-        not hold) are infinities to the products, and context().poll_status() reports them. `out` keeps its rows that belong to no sequence; without `out` they hold
-        anything."""
+        values on the device are not read here), by default all tokens and the whole page table. How the work is cut goes by them,
+        so they are worth giving, and as small as they are: 64 users of one token each (Q8_0, contexts to 8000) take 154 us without
+        max_new=1 and 115 with it, one user at 4096 keys 34 us with max_context=131072 and 8.6 with 4096.
+        Q8_0 blocks of a context with scales above 515.5 (values beyond 65500, which f16 does not hold) are infinities to the
+        products, and context().poll_status() reports them. `out` keeps its rows that belong to no sequence; without `out` they
+        hold anything."""
         dev, d = self._device, self.head_dim
         n, hq, qs = _rows(q, "q", dev, d)
         p_table = _vector(page_table, "page_table", dev, torch.int32, None)
